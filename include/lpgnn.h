@@ -745,6 +745,29 @@ lpg_status lpg_induced_fill(const int64_t *nodes, int64_t ns, const int64_t *col
                             int64_t *out_edge, void *stream);
 lpg_status lpg_sample_reset(const int64_t *nodes, int64_t ns, int64_t *local, void *stream);
 
+/* ---- layer norm over the rows of a node set (an optional layer behind every GraphConv; the
+ * reference's GCN_FC has none) ----------------------------------------------------------------
+ * y = act((x - mean) rstd w + b) per row, rstd = 1 / sqrt(var + eps) (biased variance), act = ReLU with
+ * LPG_NORM_RELU.  x / y (and dy / dx) of `dtype`, w / b (and dw / db) [D] of `wdtype`: LPG_F32, or
+ * `dtype` itself; rows contiguous, row strides in elements, any alignment of the elements' own size.
+ * w NULL = ones, b NULL = zeros.  mean / rstd fp32 [M], both or neither (forward: NULL = not kept).
+ * Statistics and sums in fp32; NaN and infinity pass through their own row.
+ * Backward: dx (NULL = not wanted), dw / db (either may be NULL; M = 0 writes zeros) from x, dy and the
+ * forward's mean / rstd; with LPG_NORM_RELU w and b must be the forward's (the mask is recomputed).
+ * dw / db need the workspace, deterministic (no atomics). */
+#define LPG_BF16 0
+#define LPG_F16 1
+#define LPG_F32 2
+#define LPG_NORM_RELU 1
+lpg_status lpg_layer_norm_fwd(int32_t dtype, int32_t wdtype, int64_t M, int64_t D, const void *x, int64_t ldx,
+                              const void *w, const void *b, float eps, int32_t flags, void *y, int64_t ldy,
+                              float *mean, float *rstd, void *stream);
+int64_t lpg_layer_norm_bwd_workspace_bytes(int64_t M, int64_t D);
+lpg_status lpg_layer_norm_bwd(int32_t dtype, int32_t wdtype, int64_t M, int64_t D, const void *x, int64_t ldx,
+                              const void *dy, int64_t lddy, const void *w, const void *b, const float *mean,
+                              const float *rstd, int32_t flags, void *dx, int64_t lddx, void *dw, void *db,
+                              void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -114,6 +114,9 @@ HEADER_SYMBOLS = (
     "lpg_colscale_f32",
     "lpg_rowcolscale_workspace_bytes",
     "lpg_rowcolscale_f32",
+    "lpg_layer_norm_fwd",
+    "lpg_layer_norm_bwd_workspace_bytes",
+    "lpg_layer_norm_bwd",
 )
 
 c_i64, c_i32, c_p = ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p
@@ -337,8 +340,19 @@ def lib() -> ctypes.CDLL:
     for nm in ("lpg_scan_i64", "lpg_sample_count", "lpg_sample_fill", "lpg_sample_dedupe", "lpg_sample_assign",
                "lpg_sample_local_ids", "lpg_induced_count", "lpg_induced_fill", "lpg_sample_reset"):
         getattr(L, nm).restype = c_i32
+    L.lpg_layer_norm_fwd.argtypes = [c_i32, c_i32, c_i64, c_i64, c_p, c_i64, c_p, c_p, ctypes.c_float, c_i32, c_p,
+                                     c_i64, c_p, c_p, c_p]
+    L.lpg_layer_norm_fwd.restype = c_i32
+    L.lpg_layer_norm_bwd_workspace_bytes.argtypes = [c_i64, c_i64]
+    L.lpg_layer_norm_bwd_workspace_bytes.restype = c_i64
+    L.lpg_layer_norm_bwd.argtypes = [c_i32, c_i32, c_i64, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_p, c_p, c_p, c_i32, c_p,
+                                     c_i64, c_p, c_p, c_p, c_p]
+    L.lpg_layer_norm_bwd.restype = c_i32
     _lib = L
     return L
+
+
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # LPG_BF16, LPG_F16, LPG_F32
 
 
 FC_RELU, FC_ACCUMULATE = 1, 2

@@ -1,0 +1,228 @@
+"""lpgnn.layer_norm on the GPU against the 64-bit reference (tests/norm_ref.py derives the bounds)."""
+import pytest
+import torch
+
+import norm_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+EPS = 1e-5
+T = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+# every lane count and vector count, both sides of each border, rows shorter than a vector and past 2048
+WIDTHS = [1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 31, 33, 64, 100, 127, 128, 200, 255, 256, 257, 333, 511, 512, 513, 768,
+          1000, 1024, 1025, 1280, 1500, 1792, 1793, 2047, 2048, 2049, 5000]
+
+
+def _inputs(M, D, dtype, wdtype, seed=0, relu=False):
+    g = torch.Generator().manual_seed(seed * 7919 + M * 31 + D)
+    n = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)
+    x = (n(M, D) * (0.5 + n(M, 1).abs()) + 2 * n(M, 1)).to(dtype)
+    w, b = (1 + 0.3 * n(D)).to(wdtype), (0.3 * n(D)).to(wdtype)
+    dy = n(M, D).to(dtype)
+    if relu:  # no gradient where the 32-bit sign of the pre-activation may differ
+        y, h, s, _ = R.norm64(x, w, b, EPS, False)
+        dy = dy * (y.abs() > R.y_error(x, w, b, y, h, s, torch.float32)).to(dtype)
+    return x, w, b, dy
+
+
+def _run(x, w, b, dy, relu, eps=EPS):
+    from lpgnn import layer_norm
+
+    ts = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    y = layer_norm(*ts, eps=eps, relu=relu)
+    return (y.detach(), *torch.autograd.grad(y, ts, dy.to(DEV)))
+
+
+def _check(x, w, b, dy, relu, out, eps=EPS):
+    y, h, s, _ = R.norm64(x, w, b, eps, relu)
+    assert R.within(out[0], y, R.y_error(x, w, b, y, h, s, x.dtype)) <= 1
+    want, bound = R.grads64(x, w, b, dy, eps, relu, x.dtype, w.dtype)
+    for got, a, e in zip(out[1:], want, bound):
+        assert R.within(got, a, e) <= 1
+
+
+@pytest.mark.parametrize("dtype,wdtype", [("fp32", "fp32"), ("bf16", "fp32"), ("bf16", "bf16"), ("fp16", "fp32"),
+                                          ("fp16", "fp16")])
+@pytest.mark.parametrize("D", WIDTHS)
+def test_forward_and_gradients(D, dtype, wdtype):
+    for M, relu in ((1, False), (3, True), (130, False), (131, True)):
+        case = _inputs(M, D, T[dtype], T[wdtype], relu=relu)
+        out = _run(*case, relu)
+        assert out[0].dtype == T[dtype] and out[1].dtype == T[dtype] and out[2].dtype == T[wdtype]
+        _check(*case, relu, out)
+
+
+@pytest.mark.parametrize("M,D,dtype", [(20011, 128, "fp32"), (20011, 333, "bf16"), (5003, 2048, "bf16")])
+def test_many_rows(M, D, dtype):
+    """More rows than the persistent grid takes at once: the row loop and the fold of all partial rows."""
+    case = _inputs(M, D, T[dtype], torch.float32)
+    out = _run(*case, False)
+    _check(*case, False, out)
+    again = _run(*case, False)
+    assert all(torch.equal(a, b) for a, b in zip(out, again))  # deterministic
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+def test_evaluation_gives_the_training_values(dtype):
+    from lpgnn import layer_norm
+
+    x, w, b, dy = _inputs(77, 200, T[dtype], torch.float32, relu=True)
+    y = _run(x, w, b, dy, True)[0]
+    with torch.no_grad():
+        assert torch.equal(layer_norm(x.to(DEV), w.to(DEV), b.to(DEV), EPS, True), y)
+    with torch.inference_mode():
+        assert torch.equal(layer_norm(x.to(DEV), w.to(DEV), b.to(DEV), EPS, True), y)
+
+
+def test_without_weight_or_bias():
+    from lpgnn import layer_norm
+
+    x, w, b, dy = _inputs(9, 40, torch.float32, torch.float32)
+    for ww, bb in ((None, None), (w, None), (None, b)):
+        ts = [None if t is None else t.to(DEV).requires_grad_(True) for t in (x, ww, bb)]
+        y = layer_norm(*ts, eps=EPS)
+        g = torch.autograd.grad(y, [t for t in ts if t is not None], dy.to(DEV))
+        yr, h, s, _ = R.norm64(x, ww, bb, EPS, False)
+        assert R.within(y.detach(), yr, R.y_error(x, ww, bb, yr, h, s, x.dtype)) <= 1
+        want, bound = R.grads64(x, ww, bb, dy, EPS, False, x.dtype, torch.float32)
+        keep = [0] + ([1] if ww is not None else []) + ([2] if bb is not None else [])
+        for got, k in zip(g, keep):
+            assert R.within(got, want[k], bound[k]) <= 1
+
+
+@pytest.mark.parametrize("need", [(True, False, False), (False, True, False), (False, False, True), (False, True, True)])
+def test_only_the_wanted_gradients(need):
+    from lpgnn import layer_norm
+
+    for D in (96, 2500):
+        x, w, b, dy = _inputs(21, D, torch.float32, torch.float32)
+        ts = [t.to(DEV).requires_grad_(k) for t, k in zip((x, w, b), need)]
+        y = layer_norm(*ts, eps=EPS)
+        g = torch.autograd.grad(y, [t for t, k in zip(ts, need) if k], dy.to(DEV))
+        want, bound = R.grads64(x, w, b, dy, EPS, False, x.dtype, w.dtype)
+        for got, a, e in zip(g, [a for a, k in zip(want, need) if k], [e for e, k in zip(bound, need) if k]):
+            assert R.within(got, a, e) <= 1
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_strides_offsets_and_shapes(dtype):
+    """Rows inside a wider buffer at an odd element offset, a transposed input, an expanded gradient, more
+    dimensions, no rows."""
+    from lpgnn import layer_norm
+
+    M, D = 37, 75
+    x, w, b, dy = _inputs(M, D, T[dtype], torch.float32)
+    wide = torch.full((M, D + 9), float("nan"), dtype=T[dtype], device=DEV)
+    wide[:, 3:3 + D] = x.to(DEV)
+    gw = torch.full((M, D + 5), float("nan"), dtype=T[dtype], device=DEV)
+    gw[:, 1:1 + D] = dy.to(DEV)
+    wd, bd = w.to(DEV).requires_grad_(True), b.to(DEV).requires_grad_(True)
+    for xv in (wide[:, 3:3 + D], x.to(DEV).t().contiguous().t()):
+        xv = xv.requires_grad_(True)
+        y = layer_norm(xv, wd, bd, EPS)
+        _check(x, w, b, dy, False, (y.detach(), *torch.autograd.grad(y, (xv, wd, bd), gw[:, 1:1 + D])))
+        xv.requires_grad_(False) if xv.is_leaf else None
+    one = dy[:1].expand(M, D)
+    xv = x.to(DEV).requires_grad_(True)
+    y = layer_norm(xv, wd, bd, EPS)
+    _check(x, w, b, one, False, (y.detach(), *torch.autograd.grad(y, (xv, wd, bd), dy[:1].to(DEV).expand(M, D))))
+    x3 = x[:36].view(4, 9, D).to(DEV)
+    assert torch.equal(layer_norm(x3, wd, bd, EPS).view(36, D), layer_norm(x.to(DEV), wd, bd, EPS)[:36])
+    empty = torch.empty(0, D, dtype=T[dtype], device=DEV, requires_grad=True)
+    y = layer_norm(empty, wd, bd, EPS)
+    gx, gww, gbb = torch.autograd.grad(y, (empty, wd, bd), torch.empty_like(y))
+    assert y.shape == (0, D) and gx.shape == (0, D) and not gww.any() and not gbb.any()
+
+
+def test_far_mean_and_constant_rows():
+    """|mean| thousands of times the spread (a one-pass variance would have no digits), and rows without
+    spread, whose h is 0 and whose gradient is scaled by 1 / sqrt(eps)."""
+    M, D = 16, 256
+    x, w, b, dy = _inputs(M, D, torch.float32, torch.float32)
+    x = (x.double() * 0.1 + 1000).float()
+    x[5] = 3.0
+    x[6] = 0.0
+    _check(x, w, b, dy, False, _run(x, w, b, dy, False))
+
+
+def test_bad_rows_stay_in_their_rows():
+    from lpgnn import layer_norm
+
+    for D in (8, 200, 2048, 3000):
+        x, w, b, _ = _inputs(9, D, torch.float32, torch.float32)
+        clean = layer_norm(x.to(DEV), w.to(DEV), b.to(DEV), EPS, True)
+        x[2, D // 2], x[4, 0], x[7, D - 1] = float("nan"), float("inf"), float("-inf")
+        y = layer_norm(x.to(DEV), w.to(DEV), b.to(DEV), EPS, True)
+        for r in range(9):
+            if r in (2, 4, 7):
+                assert torch.isnan(y[r]).all()
+            else:
+                assert torch.equal(y[r], clean[r])
+
+
+def test_gradient_against_differences():
+    """The kernel's gradients against central differences of the 64-bit definition along random directions:
+    its bound along the direction, and 1e-7 for the differences."""
+    x, w, b, dy = _inputs(6, 50, torch.float32, torch.float32)
+    got = _run(x, w, b, dy, False)[1:]
+    _, bound = R.grads64(x, w, b, dy, EPS, False, x.dtype, w.dtype)
+    f = lambda *a: (R.norm64(*a, EPS, False)[0] * dy.double()).sum()
+    ts = [t.double() for t in (x, w, b)]
+    for k in range(3):
+        d = torch.randn(ts[k].shape, generator=torch.Generator().manual_seed(k), dtype=torch.float64)
+        hi, lo = list(ts), list(ts)
+        hi[k], lo[k] = ts[k] + 1e-5 * d, ts[k] - 1e-5 * d
+        diff = (f(*hi) - f(*lo)) / 2e-5
+        assert abs(diff - (got[k].double().cpu() * d).sum()) <= (bound[k] * d.abs()).sum() + 1e-6
+
+
+def test_on_another_stream_and_in_a_graph():
+    from lpgnn import layer_norm
+
+    x, w, b, dy = (t.to(DEV) for t in _inputs(300, 128, torch.float32, torch.float32))
+    ts = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    want = layer_norm(*ts, eps=EPS)
+    want = (want.detach(), *torch.autograd.grad(want, ts, dy))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = layer_norm(*ts, eps=EPS)
+        got = (y.detach(), *torch.autograd.grad(y, ts, dy))
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del y, got
+    # captured with its backward, replayed on new inputs, eager work between the replays
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer_norm(*ts, eps=EPS)
+        held = (y.detach(), *torch.autograd.grad(y, ts, dy))
+    for k in range(3):
+        with torch.no_grad():
+            ts[0].copy_(x * (k + 1) + k)
+        graph.replay()
+        torch.cuda.synchronize()
+        e = [t.detach().clone().requires_grad_(True) for t in ts]
+        ye = layer_norm(*e, eps=EPS)
+        assert all(torch.equal(a, b) for a, b in zip(held, (ye.detach(), *torch.autograd.grad(ye, e, dy))))
+
+
+def test_refusals():
+    from lpgnn import layer_norm
+
+    x = torch.randn(4, 8, device=DEV)
+    for bad, msg in ((dict(weight=torch.ones(7, device=DEV)), "weight must be"),
+                     (dict(weight=torch.ones(8)), "weight must be"),
+                     (dict(bias=torch.ones(8, dtype=torch.float16, device=DEV)), "bias must be"),
+                     (dict(eps=-1.0), "eps")):
+        with pytest.raises(RuntimeError, match=msg):
+            layer_norm(x, **bad)
+    with pytest.raises(RuntimeError, match="share a type"):
+        layer_norm(x.half(), torch.ones(8, device=DEV), torch.ones(8, dtype=torch.float16, device=DEV))
+    with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
+        layer_norm(x.double())
+    with pytest.raises(RuntimeError, match="last dimension"):
+        layer_norm(torch.empty(3, 0, device=DEV))
+    xr = x.clone().requires_grad_(True)
+    g, = torch.autograd.grad(layer_norm(xr).sum(), xr, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
