@@ -768,6 +768,49 @@ lpg_status lpg_layer_norm_bwd(int32_t dtype, int32_t wdtype, int64_t M, int64_t 
                               const float *rstd, int32_t flags, void *dx, int64_t lddx, void *dw, void *db,
                               void *workspace, void *stream);
 
+/* ---- one AdamW step over many tensors (train.py:85-89 trains with Adam; this is its decoupled
+ * weight decay) --------------------------------------------------------------------------------
+ *   g = *grad_scale * grad (NULL = 1);  m = beta1 m + rest1 g;  v = beta2 v + rest2 g^2
+ *   p = p keep - (m / (sqrt(v) inv_root2 + eps)) rate
+ * each product and sum rounded to fp32.  At step t: rest = 1 - beta, inv_root2 = 1 / sqrt(1 - beta2^t),
+ * keep = 1 - lr weight_decay, rate = lr / (1 - beta1^t).  p and g contiguous, of `dtype` (LPG_F32 or
+ * LPG_BF16), any element alignment; m / v fp32.  No two tensors of a call may overlap.  `tensors` is a
+ * host array, read during the call; n = 0 is skipped.
+ * lpg_adamw8: the moments in 8 bits.  m8 / r8: n e4m3 numbers (OCP), ms / rs: ceil(n / 256) fp32 scales;
+ * m = m8 ms, sqrt(v) = r8 rs of the element's block of 256.  Rounding adds 16 bits of a hash of
+ * key ^ element below the kept mantissa (key: one per tensor and step).  All zeros = no history yet. */
+typedef struct {
+  float beta1, rest1, beta2, rest2, inv_root2, eps, keep, rate;
+} lpg_adamw_hyper;
+typedef struct {
+  void *p;
+  const void *g;
+  float *m, *v;
+  int64_t n;
+} lpg_adamw_tensor;
+typedef struct {
+  void *p;
+  const void *g;
+  void *m8;
+  float *ms;
+  void *r8;
+  float *rs;
+  int64_t n, key; /* key: its low 32 bits */
+} lpg_adamw8_tensor;
+typedef struct {
+  const void *p;
+  int64_t n;
+} lpg_tensor;
+lpg_status lpg_adamw(int32_t dtype, int64_t count, const lpg_adamw_tensor *tensors, const lpg_adamw_hyper *hyper,
+                     const float *grad_scale, void *stream);
+lpg_status lpg_adamw8(int32_t dtype, int64_t count, const lpg_adamw8_tensor *tensors, const lpg_adamw_hyper *hyper,
+                      const float *grad_scale, void *stream);
+/* *norm = the 2-norm of all the tensors' elements together (summed in fp64, deterministic), *scale =
+ * min(1, max_norm / (norm + 1e-6)): the clip's factor, for lpg_adamw's grad_scale.  Both on the device. */
+int64_t lpg_grad_norm_workspace_bytes(int64_t count, const lpg_tensor *tensors);
+lpg_status lpg_grad_norm(int32_t dtype, int64_t count, const lpg_tensor *tensors, double max_norm, float *norm,
+                         float *scale, void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,303 @@
+// lpgnn._host: the host side of calls that are bound by it.
+//
+// A layer norm of a small graph or the optimizer step of a small model is a few microseconds of GPU time;
+// checking the arguments, the autograd node and the launch from Python took 20 us a layer norm, 80 more
+// for its backward (a Python node in the engine's thread waits for the interpreter lock) and 40 us a step
+// over 24 tensors.  Here the same checks, the autograd node and the call of the C entry (include/lpgnn.h,
+// resolved from the library that lpgnn._lib loads) run in C++: 8, 45 and 9 us.
+//
+// Every refusal is a RuntimeError before any device work; device, stream and allocator are torch's current
+// ones of the tensors' device.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <dlfcn.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <cmath>
+#include <optional>
+#include <stdexcept>
+#include <unordered_set>
+
+#include "lpgnn.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+#define REQUIRE(cond, ...)                                   \
+  do {                                                       \
+    if (!(cond)) throw std::runtime_error(c10::str(__VA_ARGS__)); \
+  } while (0)
+
+// ------------------------------------------------------------------ the library
+struct Lib {
+  decltype(&lpg_last_error) last_error = nullptr;
+  decltype(&lpg_layer_norm_fwd) layer_norm_fwd = nullptr;
+  decltype(&lpg_layer_norm_bwd_workspace_bytes) layer_norm_bwd_workspace_bytes = nullptr;
+  decltype(&lpg_layer_norm_bwd) layer_norm_bwd = nullptr;
+  decltype(&lpg_adamw) adamw = nullptr;
+  decltype(&lpg_adamw8) adamw8 = nullptr;
+  decltype(&lpg_grad_norm_workspace_bytes) grad_norm_workspace_bytes = nullptr;
+  decltype(&lpg_grad_norm) grad_norm = nullptr;
+} L;
+
+void open(const std::string &path) {
+  void *h = dlopen(path.c_str(), RTLD_NOW | RTLD_LOCAL);  // (the one lpgnn._lib holds already)
+  REQUIRE(h, "lpgnn: ", dlerror());
+#define SYM(name)                                                               \
+  L.name = reinterpret_cast<decltype(L.name)>(dlsym(h, "lpg_" #name));          \
+  REQUIRE(L.name, "lpgnn: ", path, " has no lpg_" #name)
+  SYM(last_error);
+  SYM(layer_norm_fwd);
+  SYM(layer_norm_bwd_workspace_bytes);
+  SYM(layer_norm_bwd);
+  SYM(adamw);
+  SYM(adamw8);
+  SYM(grad_norm_workspace_bytes);
+  SYM(grad_norm);
+#undef SYM
+}
+
+void check(lpg_status st, const char *what) {  // lpgnn._lib.check
+  if (st == LPG_OK) return;
+  const char *kind = st == LPG_ERR_INVALID ? "invalid argument" : st == LPG_ERR_HIP ? "HIP error" : "unsupported";
+  throw std::runtime_error(c10::str(what, ": ", kind, ": ", L.last_error()));
+}
+
+void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+template <typename T>
+T *ptr_of(const Tensor &t) {
+  return static_cast<T *>(ptr(t));
+}
+
+int32_t code_of(at::ScalarType t) {
+  return t == at::kBFloat16 ? LPG_BF16 : t == at::kHalf ? LPG_F16 : t == at::kFloat ? LPG_F32 : -1;
+}
+
+// t as [rows, D] with contiguous rows (a copy only where its strides allow no view)
+Tensor rows(const Tensor &t) {
+  Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  return r.stride(1) == 1 && r.stride(0) >= r.size(1) ? r : r.contiguous();
+}
+
+// ------------------------------------------------------------------ layer norm
+int32_t weight_code(const Tensor &w, const Tensor &b) {
+  return w.defined() ? code_of(w.scalar_type()) : b.defined() ? code_of(b.scalar_type()) : LPG_F32;
+}
+
+Tensor norm_forward(const Tensor &x, const Tensor &w, const Tensor &b, double eps, bool relu, Tensor *stats) {
+  const c10::DeviceGuard guard(x.device());
+  const int64_t M = x.size(0), D = x.size(1);
+  Tensor y = at::empty({M, D}, x.options());
+  if (stats) *stats = at::empty({2, M}, x.options().dtype(at::kFloat));
+  float *mean = stats ? stats->data_ptr<float>() : nullptr;
+  check(L.layer_norm_fwd(code_of(x.scalar_type()), weight_code(w, b), M, D, x.data_ptr(), x.stride(0), ptr(w), ptr(b),
+                         (float)eps, relu ? LPG_NORM_RELU : 0, y.data_ptr(), D, mean, mean ? mean + M : nullptr,
+                         stream_of(x)),
+        "lpg_layer_norm_fwd");
+  return y;
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const OptTensor &weight,
+                        const OptTensor &bias, double eps, bool relu) {
+    const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    const Tensor xr = rows(x), wc = w.defined() ? w.contiguous() : w, bc = b.defined() ? b.contiguous() : b;
+    Tensor stats;
+    Tensor y = norm_forward(xr, wc, bc, eps, relu, &stats);
+    ctx->save_for_backward({xr, wc, bc, stats});
+    ctx->saved_data["relu"] = relu;
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return y.view(x.sizes());
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &stats = saved[3];
+    const c10::DeviceGuard guard(x.device());
+    const int64_t M = x.size(0), D = x.size(1);
+    const Tensor dy = rows(grads[0]);
+    Tensor dx, dw, db, ws;
+    const size_t bi = w.defined() ? 2 : 1;  // (the node's edges are its tensors: one less without a weight)
+    if (ctx->needs_input_grad(0)) dx = at::empty({M, D}, x.options());
+    if (w.defined() && ctx->needs_input_grad(1)) dw = at::empty({D}, w.options());
+    if (b.defined() && ctx->needs_input_grad(bi)) db = at::empty({D}, b.options());
+    if (dw.defined() || db.defined())
+      ws = at::empty({L.layer_norm_bwd_workspace_bytes(M, D) / 4}, x.options().dtype(at::kFloat));
+    const float *mean = stats.data_ptr<float>();
+    check(L.layer_norm_bwd(code_of(x.scalar_type()), weight_code(w, b), M, D, x.data_ptr(), x.stride(0), dy.data_ptr(),
+                           dy.stride(0), ptr(w), ptr(b), mean, mean + M,
+                           ctx->saved_data["relu"].toBool() ? LPG_NORM_RELU : 0, ptr(dx), D, ptr(dw), ptr(db), ptr(ws),
+                           stream_of(x)),
+          "lpg_layer_norm_bwd");
+    if (dx.defined()) dx = dx.view(ctx->saved_data["shape"].toIntVector());
+    return {dx, dw, db, Tensor(), Tensor()};
+  }
+};
+
+Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double eps, bool relu) {
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  REQUIRE(x.is_cuda(), "lpgnn layer_norm: runs on a HIP device only (no CPU path)");
+  REQUIRE(code_of(x.scalar_type()) >= 0, "lpgnn layer_norm: x must be float32, bfloat16 or float16, got ",
+          x.scalar_type());
+  REQUIRE(x.dim() > 0 && x.size(-1) > 0, "lpgnn layer_norm: x needs a last dimension to normalise, got shape ", x.sizes());
+  REQUIRE(eps >= 0, "lpgnn layer_norm: eps must not be negative, got ", eps);
+  for (const Tensor &p : {w, b}) {
+    if (!p.defined()) continue;
+    const char *name = p.is_same(w) ? "weight" : "bias";
+    REQUIRE(p.dim() == 1 && p.size(0) == x.size(-1) && p.device() == x.device(), "lpgnn layer_norm: ", name, " must be [",
+            x.size(-1), "] on ", x.device(), ", got ", p.sizes(), " on ", p.device());
+    REQUIRE(p.scalar_type() == at::kFloat || p.scalar_type() == x.scalar_type(), "lpgnn layer_norm: ", name,
+            " must be float32 or ", x.scalar_type(), ", got ", p.scalar_type());
+  }
+  REQUIRE(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
+          "lpgnn layer_norm: weight and bias must share a type, got ", w.scalar_type(), " and ", b.scalar_type());
+  const auto grad = [](const Tensor &t) { return t.defined() && t.requires_grad(); };
+  if (at::GradMode::is_enabled() && (grad(x) || grad(w) || grad(b))) return LayerNorm::apply(x, weight, bias, eps, relu);
+  return norm_forward(rows(x), w.defined() ? w.contiguous() : w, b.defined() ? b.contiguous() : b, eps, relu, nullptr)
+      .view(x.sizes());
+}
+
+// ------------------------------------------------------------------ many tensors
+using Tensors = std::vector<Tensor>;
+
+// `ts` beside the parameters `ps`: as many, one type, the parameters' device, contiguous, their sizes (or,
+// scales, one number a block of 256)
+void same(const char *what, const char *name, const Tensors &ts, const Tensors &ps, at::ScalarType type,
+          bool blocks = false) {
+  REQUIRE(ts.size() == ps.size(), "lpgnn ", what, ": ", ps.size(), " params and ", ts.size(), " ", name);
+  for (size_t i = 0; i < ts.size(); ++i) {
+    const Tensor &t = ts[i];
+    REQUIRE(t.scalar_type() == type, "lpgnn ", what, ": ", name, " must be ", type, ", got ", t.scalar_type());
+    REQUIRE(t.device() == ps[0].device(), "lpgnn ", what, ": ", name, " must be on the parameters' device");
+    REQUIRE(t.layout() == at::kStrided && t.is_contiguous(), "lpgnn ", what, ": ", name, " must be contiguous");
+    const int64_t n = ps[i].numel();
+    REQUIRE(t.numel() == (blocks ? (n + 255) / 256 : n), "lpgnn ", what, ": ", name,
+            " do not have the parameters' sizes");
+  }
+}
+
+int32_t params(const char *what, const Tensors &ps) {
+  REQUIRE(ps[0].is_cuda(), "lpgnn ", what, ": runs on a HIP device only (no CPU path)");
+  const auto type = ps[0].scalar_type();
+  REQUIRE(type == at::kFloat || type == at::kBFloat16, "lpgnn ", what, ": parameters must be float32 or bfloat16, got ",
+          type);
+  same(what, "params", ps, ps, type);
+  return code_of(type);
+}
+
+void once(const char *what, const Tensors &ps) {
+  std::unordered_set<void *> seen;
+  for (const Tensor &t : ps)
+    REQUIRE(t.numel() == 0 || seen.insert(t.data_ptr()).second, "lpgnn ", what, ": a parameter is in the list twice");
+}
+
+lpg_adamw_hyper hyper(const char *what, int64_t step, double lr, std::pair<double, double> betas, double eps,
+                      double weight_decay) {
+  const double b1 = betas.first, b2 = betas.second;
+  REQUIRE(step >= 1, "lpgnn ", what, ": step counts from 1, got ", step);
+  REQUIRE(lr >= 0 && eps >= 0 && weight_decay >= 0 && b1 >= 0 && b1 < 1 && b2 >= 0 && b2 < 1, "lpgnn ", what,
+          ": need lr, eps, weight_decay >= 0 and 0 <= betas < 1, got lr=", lr, " betas=(", b1, ", ", b2, ") eps=", eps,
+          " weight_decay=", weight_decay);
+  return {(float)b1, (float)(1 - b1), (float)b2, (float)(1 - b2), (float)(1 / std::sqrt(1 - std::pow(b2, (double)step))),
+          (float)eps, (float)(1 - lr * weight_decay), (float)(lr / (1 - std::pow(b1, (double)step)))};
+}
+
+const float *scale_ptr(const char *what, const OptTensor &s, const Tensors &ps) {
+  if (!s) return nullptr;
+  REQUIRE(s->scalar_type() == at::kFloat && s->numel() == 1 && s->device() == ps[0].device(), "lpgnn ", what,
+          ": grad_scale must be one float32 number on the parameters' device");
+  return s->data_ptr<float>();
+}
+
+void adamw_step(const Tensors &ps, const Tensors &gs, const Tensors &ms, const Tensors &vs, int64_t step, double lr,
+                std::pair<double, double> betas, double eps, double weight_decay, const OptTensor &grad_scale) {
+  const char *what = "adamw_step";
+  const lpg_adamw_hyper h = hyper(what, step, lr, betas, eps, weight_decay);
+  if (ps.empty()) return;
+  const int32_t type = params(what, ps);
+  once(what, ps);
+  same(what, "grads", gs, ps, ps[0].scalar_type());
+  same(what, "exp_avgs", ms, ps, at::kFloat);
+  same(what, "exp_avg_sqs", vs, ps, at::kFloat);
+  const float *scale = scale_ptr(what, grad_scale, ps);
+  std::vector<lpg_adamw_tensor> tab(ps.size());
+  for (size_t i = 0; i < ps.size(); ++i)
+    tab[i] = {ps[i].data_ptr(), gs[i].data_ptr(), ptr_of<float>(ms[i]), ptr_of<float>(vs[i]), ps[i].numel()};
+  const c10::DeviceGuard guard(ps[0].device());
+  check(L.adamw(type, (int64_t)tab.size(), tab.data(), &h, scale, stream_of(ps[0])), "lpg_adamw");
+}
+
+// The 32-bit integer hash of the kernels' random bits (fc_common.h lowbias32), for the rounding key of a
+// tensor: of the seed, the step and the tensor's place in the list.
+uint32_t mix(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0x7feb352du;
+  x ^= x >> 15;
+  x *= 0x846ca68bu;
+  return x ^ (x >> 16);
+}
+uint32_t step_key(int64_t step, uint64_t seed) {
+  return mix((uint32_t)seed ^ mix((uint32_t)(seed >> 32) ^ mix((uint32_t)step)));
+}
+int64_t rounding_key(int64_t place, int64_t step, uint64_t seed) {
+  return mix(step_key(step, seed) + 0x9e3779b9u * (uint32_t)(place + 1));
+}
+
+void adamw_step_8bit(const Tensors &ps, const Tensors &gs, const Tensors &m8, const Tensors &ms, const Tensors &r8,
+                     const Tensors &rs, const std::optional<std::vector<int64_t>> &places, uint64_t seed, int64_t step,
+                     double lr, std::pair<double, double> betas, double eps, double weight_decay,
+                     const OptTensor &grad_scale) {
+  const char *what = "adamw_step_8bit";
+  const lpg_adamw_hyper h = hyper(what, step, lr, betas, eps, weight_decay);
+  if (ps.empty()) return;
+  const int32_t type = params(what, ps);
+  once(what, ps);
+  REQUIRE(!places || places->size() == ps.size(), "lpgnn ", what, ": ", ps.size(), " params and ", places->size(),
+          " places");
+  same(what, "grads", gs, ps, ps[0].scalar_type());
+  same(what, "m8", m8, ps, at::kFloat8_e4m3fn);
+  same(what, "m_scales", ms, ps, at::kFloat, true);
+  same(what, "r8", r8, ps, at::kFloat8_e4m3fn);
+  same(what, "r_scales", rs, ps, at::kFloat, true);
+  const float *scale = scale_ptr(what, grad_scale, ps);
+  std::vector<lpg_adamw8_tensor> tab(ps.size());
+  for (size_t i = 0; i < ps.size(); ++i)
+    tab[i] = {ps[i].data_ptr(),      gs[i].data_ptr(), m8[i].data_ptr(), ptr_of<float>(ms[i]),
+              r8[i].data_ptr(), ptr_of<float>(rs[i]), ps[i].numel(),    rounding_key(places ? (*places)[i] : (int64_t)i, step, seed)};
+  const c10::DeviceGuard guard(ps[0].device());
+  check(L.adamw8(type, (int64_t)tab.size(), tab.data(), &h, scale, stream_of(ps[0])), "lpg_adamw8");
+}
+
+std::pair<Tensor, Tensor> clip_scale(const Tensors &gs, double max_norm) {
+  const char *what = "clip_scale";
+  REQUIRE(!gs.empty(), "lpgnn clip_scale: no gradients");
+  REQUIRE(max_norm >= 0, "lpgnn clip_scale: max_norm must not be negative, got ", max_norm);
+  const int32_t type = params(what, gs);
+  std::vector<lpg_tensor> tab(gs.size());
+  for (size_t i = 0; i < gs.size(); ++i) tab[i] = {gs[i].data_ptr(), gs[i].numel()};
+  const c10::DeviceGuard guard(gs[0].device());
+  Tensor out = at::empty({2}, gs[0].options().dtype(at::kFloat));
+  Tensor ws = at::empty({L.grad_norm_workspace_bytes((int64_t)tab.size(), tab.data()) / 8},
+                        out.options().dtype(at::kDouble));
+  float *o = out.data_ptr<float>();
+  check(L.grad_norm(type, (int64_t)tab.size(), tab.data(), max_norm, o, o + 1, ws.data_ptr(), stream_of(out)),
+        "lpg_grad_norm");
+  return {out[0], out[1]};
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_host, m) {
+  m.def("open", &open);
+  m.def("layer_norm", &layer_norm);
+  m.def("rounding_key", &rounding_key);
+  m.def("adamw_step", &adamw_step);
+  m.def("adamw_step_8bit", &adamw_step_8bit);
+  m.def("clip_scale", &clip_scale);
+}

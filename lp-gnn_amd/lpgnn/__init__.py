@@ -6,6 +6,7 @@ Public surface (mirrors the reference's names):
   loader: NeighborLoader, NeighborSampler (device k-hop sampling)
   sparse: BipartiteCSR (the batch's edge_index), spmm
   norm:  layer_norm, LayerNorm (GCN_FC(..., norm="layer"))
+  optim: AdamW (32- or 8-bit state), adamw_step, adamw_step_8bit, clip_scale
   ops:   torch.ops.lpgnn.spmm_sum (torch_sparse's spmm_sum schema + autograd)
   val:   inference_gnn, accuracy, model_inference_with_batch
   train: balanced, labels_to_balanced_weights, train_step, make_optimizer
@@ -16,12 +17,13 @@ from .arch import GCN_FC, GraphConv, GraphConvTwoDirection, Linear, add_knowledg
 from .data import BipartiteBatch, MyToBipartite, UnipartiteData, batch_to, lp_to_unipartite
 from .loader import NeighborLoader, NeighborSampler
 from .norm import LayerNorm, layer_norm
+from . import optim
 from . import ops  # registers torch.ops.lpgnn.spmm_sum
 
 __all__ = [
     "BipartiteCSR", "CSR", "spmm", "GCN_FC", "GraphConv", "GraphConvTwoDirection", "Linear",
     "add_knowledge", "build_model", "BipartiteBatch", "MyToBipartite", "UnipartiteData", "batch_to",
-    "lp_to_unipartite", "NeighborLoader", "NeighborSampler", "LayerNorm", "layer_norm",
+    "lp_to_unipartite", "NeighborLoader", "NeighborSampler", "LayerNorm", "layer_norm", "optim",
 ]
 
 

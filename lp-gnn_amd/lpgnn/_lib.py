@@ -117,6 +117,10 @@ HEADER_SYMBOLS = (
     "lpg_layer_norm_fwd",
     "lpg_layer_norm_bwd_workspace_bytes",
     "lpg_layer_norm_bwd",
+    "lpg_adamw",
+    "lpg_adamw8",
+    "lpg_grad_norm_workspace_bytes",
+    "lpg_grad_norm",
 )
 
 c_i64, c_i32, c_p = ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p
@@ -135,6 +139,11 @@ class LpgFc16Call(ctypes.Structure):
                 ("dropout_p", ctypes.c_float), ("seed", ctypes.c_uint64), ("row_offset", c_i64), ("row_keys", c_p),
                 ("mask_out", c_p), ("ldmo", c_i64), ("Y", c_p), ("ldy", c_i64), ("mask_in", c_p), ("ldmi", c_i64),
                 ("scale", ctypes.c_float), ("db", c_p), ("db_workspace", c_p)]
+
+
+class LpgAdamwHyper(ctypes.Structure):
+    """include/lpgnn.h lpg_adamw_hyper."""
+    _fields_ = [(k, ctypes.c_float) for k in ("beta1", "rest1", "beta2", "rest2", "inv_root2", "eps", "keep", "rate")]
 
 
 _lib = None
@@ -348,11 +357,34 @@ def lib() -> ctypes.CDLL:
     L.lpg_layer_norm_bwd.argtypes = [c_i32, c_i32, c_i64, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_p, c_p, c_p, c_i32, c_p,
                                      c_i64, c_p, c_p, c_p, c_p]
     L.lpg_layer_norm_bwd.restype = c_i32
+    # tensor tables: host arrays of structures of 8-byte fields, passed as int64 arrays
+    L.lpg_adamw.argtypes = [c_i32, c_i64, c_p, ctypes.POINTER(LpgAdamwHyper), c_p, c_p]
+    L.lpg_adamw.restype = c_i32
+    L.lpg_adamw8.argtypes = L.lpg_adamw.argtypes
+    L.lpg_adamw8.restype = c_i32
+    L.lpg_grad_norm_workspace_bytes.argtypes = [c_i64, c_p]
+    L.lpg_grad_norm_workspace_bytes.restype = c_i64
+    L.lpg_grad_norm.argtypes = [c_i32, c_i64, c_p, ctypes.c_double, c_p, c_p, c_p, c_p]
+    L.lpg_grad_norm.restype = c_i32
     _lib = L
     return L
 
 
-DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # LPG_BF16, LPG_F16, LPG_F32
+_host = None
+
+
+def host():
+    """lpgnn._host (csrc/host.cpp): the C++ host side of the latency-bound calls, on the library of lib()."""
+    global _host
+    if _host is None:
+        try:
+            from . import _host as h
+        except ImportError as e:
+            raise RuntimeError(f"lpgnn._host is not built ({e}); run `make -C lp-gnn_amd` or __graft_entry__.build()")
+        lib()
+        h.open(LIB_PATH)
+        _host = h
+    return _host
 
 
 FC_RELU, FC_ACCUMULATE = 1, 2
