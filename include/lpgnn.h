@@ -811,6 +811,25 @@ int64_t lpg_grad_norm_workspace_bytes(int64_t count, const lpg_tensor *tensors);
 lpg_status lpg_grad_norm(int32_t dtype, int64_t count, const lpg_tensor *tensors, double max_norm, float *norm,
                          float *scale, void *workspace, void *stream);
 
+/* ---- the fully connected layer in 8-bit integers (evaluation) -----------------------------------
+ * lpg_quant_i8: row i of [x | x2] (dtype, K1 and K2 columns, row strides ldx / ldx2, K2 = 0: x2 unused)
+ * as int8: q = round_half_even(127 x / top), top = the row's largest |x|, exactly (no 32-bit quotient
+ * decides a border), scale[i] = top / 127; q [M, ldq], its columns from K1 + K2 to ldq zero (ldq a
+ * multiple of 128).  A row below 2^-100 counts as zero; one with a NaN or an infinity gets the scale NaN.
+ * lpg_fc_i8: y = act((sum_k q[m,k] w[n,k]) scale[m] wscale[n] + bias[n]), the sum exact in 32-bit
+ * integers, y of `dtype` [M, N]; w int8 [N, ldw], ldw a multiple of 16, 16-byte aligned, each row readable
+ * to K rounded up to 16 (what lies past K meets zeros of q); K <= 131072; bias NULL = 0; flags: LPG_FC_RELU.
+ * lpg_fc_i8_rows: both in one launch for a few rows (M <= 8, and M codes of K bytes rounded up to
+ * 1024 within 48 KiB, else LPG_ERR_UNSUPPORTED): no q, no workspace. */
+lpg_status lpg_quant_i8(int32_t dtype, int64_t M, int64_t K1, const void *x, int64_t ldx, int64_t K2, const void *x2,
+                        int64_t ldx2, int8_t *q, int64_t ldq, float *scale, void *stream);
+lpg_status lpg_fc_i8(int32_t dtype, int64_t M, int64_t N, int64_t K, const int8_t *q, int64_t ldq, const float *scale,
+                     const int8_t *w, int64_t ldw, const float *wscale, const float *bias, int32_t flags, void *y,
+                     int64_t ldy, void *stream);
+lpg_status lpg_fc_i8_rows(int32_t dtype, int64_t M, int64_t N, int64_t K1, const void *x, int64_t ldx, int64_t K2,
+                          const void *x2, int64_t ldx2, const int8_t *w, int64_t ldw, const float *wscale,
+                          const float *bias, int32_t flags, void *y, int64_t ldy, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,545 @@
+// The fully connected layer in 8-bit integers, for evaluation:
+//
+//   top_m = max_k |x_mk|,  q_mk = round_half_even(127 x_mk / top_m),  x = [x1 | x2] (aggregate | own features)
+//   y_mn = act((sum_k q_mk w_nk) (top_m / 127) ws_n + b_n)
+//
+// w int8 with a scale ws an output channel, quantised ahead.  The sum is exact (32-bit integers, K <=
+// 131072), so every variant below gives the same bits.
+//
+// The quotient decides borders of whole numbers, so it is decided exactly: x (127 / top) in fp32 is off by
+// less than 127 * 2^-23 < 2^-15.9; where it lies within 2^-15 of a border between two codes (one element
+// in 16000), the vector is done again in fp64, whose correctly rounded 127 x / top is never on the wrong
+// side of a border (two fp32 numbers' quotient is either that border or at least 2^-26 away from it).
+//
+// quant_rows: one wave a row, two passes over it (the second from cache).  HBM-bound: x in, q out.
+// fc_i8: MFMA-bound (v_mfma_i32_16x16x64_i8), the k loop of the 16-bit kernel (fc_bf16.hip fc_bf16_p) on
+// bytes: 128-byte k tiles staged by buffer_load ... lds into a swizzled image, two buffers, one barrier a
+// tile in its middle, fragment reads one half tile ahead, transposed fragments (W x A^T: a lane holds four
+// consecutive columns of one row).
+// fc_i8_rows: a few rows (M <= 8) are bound by w's bytes and by latency: every block quantises the rows
+// into LDS itself (no second launch, no q in memory), its first loads of w in flight meanwhile, then a
+// wave a column, 16 bytes of w a lane, v_dot4.
+#include "common.h"
+#include "fc_common.h"
+
+#include <type_traits>
+
+namespace lpg {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int BK = 128;  // bytes of a k tile
+constexpr float kTiny = 0x1p-100f;
+
+__device__ __forceinline__ int swz(int row, int chunk) { return chunk ^ ((row >> 1) & 7); }
+
+// The row's factor 127 / top and scale top / 127, from the bits of its largest |x| (as unsigned numbers, so
+// a NaN or an infinity is on top).
+struct RowScale {
+  float top, inv, scale;
+  __device__ __forceinline__ explicit RowScale(uint32_t bits) {
+    top = __uint_as_float(bits);
+    const bool bad = bits >= 0x7f800000u, live = !bad && top >= kTiny;
+    inv = live ? 127.f / top : 0.f;
+    scale = bad ? __uint_as_float(0x7fc00000u) : (live ? top / 127.f : 0.f);
+  }
+};
+
+// n codes of f (inv = 0: zeros, whatever f holds), packed four to a word
+template <int N>
+__device__ __forceinline__ void quant(const float (&f)[N], const RowScale &s, uint32_t (&q)[(N + 3) / 4]) {
+  int c[N];
+  bool near = false;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float t = f[j] * s.inv, r = __builtin_rintf(t);
+    near |= fabsf(fabsf(t - r) - 0.5f) < 0x1p-15f;
+    c[j] = (int)r;
+  }
+  if (near) {
+#pragma unroll 1
+    for (int j = 0; j < N; ++j) {
+      const double t = (double)f[j] * 127.0 / (double)s.top;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i == j) c[i] = (int)__builtin_rint(t);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < (N + 3) / 4; ++j) q[j] = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) q[j / 4] |= ((uint32_t)(s.inv == 0.f ? 0 : c[j]) & 0xffu) << (8 * (j & 3));
+}
+
+template <typename T>
+__device__ __forceinline__ void ldv(const T *p, float (&f)[16 / sizeof(T)]) {
+  T t[16 / sizeof(T)];
+  __builtin_memcpy(t, p, 16);
+#pragma unroll
+  for (int j = 0; j < (int)(16 / sizeof(T)); ++j) f[j] = (float)t[j];
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+  return v;
+}
+
+// the largest |x| bits of the n elements at p, taken by threads t of nt
+template <typename T>
+__device__ __forceinline__ uint32_t part_max(const T *p, int n, int t, int nt) {
+  constexpr int V = 16 / sizeof(T);
+  uint32_t top = 0;
+  const int nv = n / V;
+  for (int i = t; i < nv; i += nt) {
+    float f[V];
+    ldv(p + i * V, f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) top = max(top, abs_bits(f[j]));
+  }
+  const int at = nv * V + t;
+  if (at < n) top = max(top, abs_bits((float)p[at]));  // (fewer than V <= nt are left)
+  return top;
+}
+
+// ... and their codes, to q (any alignment)
+template <typename T>
+__device__ __forceinline__ void part_quant(const T *p, int n, int t, int nt, const RowScale &s, int8_t *q) {
+  constexpr int V = 16 / sizeof(T);
+  const int nv = n / V;
+  for (int i = t; i < nv; i += nt) {
+    float f[V];
+    uint32_t o[V / 4];
+    ldv(p + i * V, f);
+    quant<V>(f, s, o);
+    __builtin_memcpy(q + i * V, o, V);
+  }
+  const int at = nv * V + t;
+  if (at < n) {
+    const float f[1] = {(float)p[at]};
+    uint32_t o[1];
+    quant<1>(f, s, o);
+    q[at] = (int8_t)o[0];
+  }
+}
+
+struct QuantArgs {
+  int64_t M, ldx, ldx2, ldq;
+  int K1, K2;
+  const void *x, *x2;
+  int8_t *q;
+  float *scale;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void quant_rows(QuantArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.M) return;
+  const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+  const T *x2 = a.K2 ? static_cast<const T *>(a.x2) + row * a.ldx2 : nullptr;
+  int8_t *q = a.q + row * a.ldq;
+  uint32_t top = part_max(x, a.K1, lane, 64);
+  if (a.K2) top = max(top, part_max(x2, a.K2, lane, 64));
+  const RowScale s(wave_max(top));
+  part_quant(x, a.K1, lane, 64, s, q);
+  if (a.K2) part_quant(x2, a.K2, lane, 64, s, q + a.K1);
+  for (int64_t k = a.K1 + a.K2 + lane; k < a.ldq; k += 64) q[k] = 0;
+  if (lane == 0) a.scale[row] = s.scale;
+}
+
+struct FcArgs {
+  int64_t M, N, ldq, ldw, ldy;
+  int K;
+  const int8_t *q, *w;
+  const float *scale, *wscale, *bias;
+  void *y;
+  int64_t mt, nt;
+  int relu;
+};
+
+__device__ __forceinline__ float finish(int acc, float s, float ws, float b, int relu) {
+  const float v = ((float)acc * s) * ws + b;
+  return relu && v < 0.f ? 0.f : v;  // (a NaN stays one)
+}
+
+// WM x WN waves, each FM x FN fragments of 16 x 16.
+template <typename T, int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
+  constexpr int NW = WM * WN;
+  constexpr int BM = WM * FM * 16, BN = WN * FN * 16;
+  constexpr int A_BYTES = BM * BK, TILE_BYTES = A_BYTES + BN * BK;
+  constexpr int PA = BM / 8, PT = PA + BN / 8, PPW = PT / NW;  // 1-KiB pieces: A, all, a wave
+  static_assert(PA % NW == 0 && PT % NW == 0 && NW % 2 == 0 && PA % 2 == 0, "whole pieces a wave, of one row parity");
+  constexpr int EP_PITCH = FN * 16 * 2 + 16;  // 16-bit outputs: the epilogue's image
+  constexpr int EP_BYTES = sizeof(T) == 2 ? NW * FM * 16 * EP_PITCH : 0;
+  constexpr int SMEM = 2 * TILE_BYTES > EP_BYTES ? 2 * TILE_BYTES : EP_BYTES;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[SMEM];
+
+  // XCD-aware order: the blocks of one XCD take a contiguous range of (m, n) tiles
+  const int64_t nwg = a.mt * a.nt, bid = blockIdx.x, xcd = bid % 8, q8 = nwg / 8, rr = nwg % 8;
+  const int64_t wgid = (xcd < rr ? xcd * (q8 + 1) : rr * (q8 + 1) + (xcd - rr) * q8) + bid / 8;
+  const int64_t m0 = wgid / a.nt * BM, n0 = wgid % a.nt * BN;
+  const int64_t mrows = a.M - m0 < BM ? a.M - m0 : BM, ncols = a.N - n0 < BN ? a.N - n0 : BN;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int nk = (a.K + BK - 1) / BK, k16 = (a.K + 15) / 16 * 16;
+
+  // Descriptors from row m0 of q / row n0 of w, ending with the block's last row: the lane offsets of rows
+  // past it are past the range and read zeros.  q's rows hold zeros from K to the tile's end; a row of w
+  // may end before the tile does (the lanes of those chunks get an offset past the range).
+  const uint64_t pa = (uint64_t)(a.q + m0 * a.ldq), pw = (uint64_t)(a.w + n0 * a.ldw);
+  const uint32_t na = (uint32_t)((mrows - 1) * a.ldq + nk * BK), nw = (uint32_t)((ncols - 1) * a.ldw + k16);
+  uint32_t vo[PPW];
+#pragma unroll
+  for (int p = 0; p < PPW; ++p) {
+    const int q = wave + NW * p;
+    const int row = (q < PA ? q : q - PA) * 8 + (lane >> 3);
+    vo[p] = (uint32_t)(row * (q < PA ? a.ldq : a.ldw) + swz(row, lane & 7) * 16);
+  }
+  const int chunk_at = swz((wave & 1) * 8 + (lane >> 3), lane & 7) * 16;  // of all this wave's pieces
+  auto stage = [&](int b, int t) {
+    const bool ok = t < nk;  // past the last tile: the same instructions with an empty range
+    t = ok ? t : nk - 1;
+    unsigned char *base = smem + b * TILE_BYTES;
+    const uint32_t ra = ok ? na : 0u, rw = ok ? nw : 0u;
+    const bool in = chunk_at < k16 - t * BK;
+#pragma unroll
+    for (int p = 0; p < PPW; ++p) {
+      const int q = wave + NW * p;
+      if (p < PA / NW) dma16(pa, ra, base + q * 1024, vo[p], t * BK);
+      else dma16(pw, rw, base + q * 1024, in ? vo[p] : 0x7fffff00u, t * BK);
+    }
+  };
+
+  i32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+
+  const int fr = lane & 15, fq = lane >> 4;
+  auto rd = [&](int b, int s, i32x4(&av)[FM], i32x4(&bv)[FN]) {  // half s (64 k) of buffer b
+    const unsigned char *As = smem + b * TILE_BYTES, *Bs = As + A_BYTES;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int row = wm * FM * 16 + i * 16 + fr;
+      av[i] = *reinterpret_cast<const i32x4 *>(As + row * BK + swz(row, s * 4 + fq) * 16);
+    }
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int row = wn * FN * 16 + j * 16 + fr;
+      bv[j] = *reinterpret_cast<const i32x4 *>(Bs + row * BK + swz(row, s * 4 + fq) * 16);
+    }
+  };
+  auto mma = [&](const i32x4(&av)[FM], const i32x4(&bv)[FN]) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bv[j], av[i], acc[i][j], 0, 0, 0);
+  };
+  auto barrier = [&]() {  // this wave's DMA landed and its fragment reads returned; then all waves
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  i32x4 a0[FM], b0[FN], a1[FM], b1[FN];
+  stage(0, 0);
+  barrier();
+  if (nk > 1) stage(1, 1);
+  rd(0, 0, a0, b0);
+  constexpr int NR = FM + FN, NM = FM * FN;
+  for (int t = 0; t + 1 < nk; ++t) {
+    const int b = t & 1;
+    rd(b, 1, a1, b1);
+    mma(a0, b0);
+    barrier();  // tile t + 1 landed everywhere; every wave is done reading buffer b
+    stage(b, t + 2);
+    rd(b ^ 1, 0, a0, b0);
+    mma(a1, b1);
+    if constexpr (NM > PPW + NR) {  // DMA pieces, then the next tile's reads, one a MFMA
+#pragma unroll
+      for (int k = 0; k < PPW; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < NR; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, NM - PPW - NR, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  rd((nk - 1) & 1, 1, a1, b1);
+  mma(a0, b0);
+  mma(a1, b1);
+  // the image reuses the tile buffers: the last (empty) DMA has landed, every wave is past its reads
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+
+  // a lane holds row 16 i + fr, columns 16 j + 4 fq .. + 3 of its wave's part
+  const int64_t r0 = m0 + wm * FM * 16, c0 = n0 + wn * FN * 16;
+  float ws[FN][4], bb[FN][4];
+#pragma unroll
+  for (int j = 0; j < FN; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t c = c0 + j * 16 + fq * 4 + r;
+      ws[j][r] = c < a.N ? a.wscale[c] : 0.f;
+      bb[j][r] = a.bias && c < a.N ? a.bias[c] : 0.f;
+    }
+  T *y = static_cast<T *>(a.y);
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int64_t row = r0 + i * 16 + fr;
+      const float s = row < a.M ? a.scale[row] : 0.f;
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int64_t c = c0 + j * 16 + fq * 4;
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = finish(acc[i][j][r], s, ws[j][r], bb[j][r], a.relu);
+        if (row < a.M && c + 4 <= a.N) {
+          __builtin_memcpy(y + row * a.ldy + c, v, 16);
+        } else if (row < a.M) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (c + r < a.N) y[row * a.ldy + c + r] = v[r];
+        }
+      }
+    }
+  } else {
+    // through LDS, so that rows leave as 16-byte stores
+    unsigned char *img = smem + wave * (FM * 16 * EP_PITCH);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int64_t row = r0 + i * 16 + fr;
+      const float s = row < a.M ? a.scale[row] : 0.f;
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        T v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = (T)finish(acc[i][j][r], s, ws[j][r], bb[j][r], a.relu);
+        uint2 o;
+        __builtin_memcpy(&o, v, 8);
+        *reinterpret_cast<uint2 *>(img + (i * 16 + fr) * EP_PITCH + (j * 16 + fq * 4) * 2) = o;
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    constexpr int CPR = FN * 16 / 8;  // 16-byte chunks a row
+    const bool al = (a.ldy & 7) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
+#pragma unroll
+    for (int it = 0; it < FM * 16 * CPR / 64; ++it) {
+      const int k = it * 64 + lane, lr = k / CPR, ch = k % CPR;
+      const int64_t row = r0 + lr, c = c0 + ch * 8;
+      const u32x4 v = *reinterpret_cast<const u32x4 *>(img + lr * EP_PITCH + ch * 16);
+      if (row >= a.M || c >= a.N) continue;
+      T *p = y + row * a.ldy + c;
+      if (c + 8 <= a.N) {
+        if (al) __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(p));
+        else __builtin_memcpy(p, &v, 16);
+      } else {
+        T e[8];
+        __builtin_memcpy(e, &v, 16);
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (c + r < a.N) p[r] = e[r];
+      }
+    }
+  }
+}
+
+struct RowsArgs {
+  int64_t N, ldx, ldx2, ldw, ldy;
+  int M, K1, K2;
+  const void *x, *x2;
+  const int8_t *w;
+  const float *wscale, *bias;
+  void *y;
+  int relu;
+};
+
+constexpr int kRows = 8;                // the most rows of fc_i8_rows
+constexpr int kRowsBytes = 48 * 1024;   // ... and the most bytes of their codes in LDS
+
+template <typename T, int RM>
+__global__ __launch_bounds__(256) void fc_i8_rows(RowsArgs a) {
+  extern __shared__ __attribute__((aligned(16))) int8_t qs[];  // RM rows of kp bytes
+  __shared__ uint32_t red[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int K = a.K1 + a.K2, k16 = (K + 15) / 16, kp = (k16 * 16 + 1023) / 1024 * 1024;
+  const int64_t n = (int64_t)blockIdx.x * 4 + wave;
+  const i32x4 *w = reinterpret_cast<const i32x4 *>(a.w + (n < a.N ? n : a.N - 1) * a.ldw);
+  // the first chunks of this wave's column, in flight while the rows are quantised
+  constexpr int P = 4;
+  i32x4 pre[P];
+#pragma unroll
+  for (int u = 0; u < P; ++u) pre[u] = u * 64 + lane < k16 ? w[u * 64 + lane] : i32x4{0, 0, 0, 0};
+  float scale[RM];
+#pragma unroll
+  for (int m = 0; m < RM; ++m) {
+    if (m < a.M) {
+      const T *x = static_cast<const T *>(a.x) + m * a.ldx;
+      const T *x2 = a.K2 ? static_cast<const T *>(a.x2) + m * a.ldx2 : nullptr;
+      uint32_t top = part_max(x, a.K1, (int)threadIdx.x, 256);
+      if (a.K2) top = max(top, part_max(x2, a.K2, (int)threadIdx.x, 256));
+      top = wave_max(top);
+      __syncthreads();
+      if (lane == 0) red[wave] = top;
+      __syncthreads();
+      const RowScale s(max(max(red[0], red[1]), max(red[2], red[3])));
+      int8_t *q = qs + m * kp;
+      part_quant(x, a.K1, (int)threadIdx.x, 256, s, q);
+      if (a.K2) part_quant(x2, a.K2, (int)threadIdx.x, 256, s, q + a.K1);
+      for (int k = K + (int)threadIdx.x; k < kp; k += 256) q[k] = 0;
+      scale[m] = s.scale;
+    }
+  }
+  __syncthreads();
+  int acc[RM];
+#pragma unroll
+  for (int m = 0; m < RM; ++m) acc[m] = 0;
+  const auto dot = [&](i32x4 v, int c) {
+#pragma unroll
+    for (int m = 0; m < RM; ++m)
+      if (m < a.M) {
+        const i32x4 q = *reinterpret_cast<const i32x4 *>(qs + m * kp + c * 16);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[m] = __builtin_amdgcn_sdot4(v[r], q[r], acc[m], false);
+      }
+  };
+#pragma unroll
+  for (int u = 0; u < P; ++u)
+    if (u * 64 < k16) dot(pre[u], u * 64 + lane);  // (chunks past k16 are zeros; q is padded to whole kilobytes)
+  for (int c = P * 64 + lane; c < k16; c += 64) dot(w[c], c);
+#pragma unroll
+  for (int m = 0; m < RM; ++m) {
+    if (m >= a.M) continue;
+    int v = acc[m];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if (lane == 0 && n < a.N)
+      static_cast<T *>(a.y)[m * a.ldy + n] = (T)finish(v, scale[m], a.wscale[n], a.bias ? a.bias[n] : 0.f, a.relu);
+  }
+}
+
+template <typename T, int WM, int WN, int FM, int FN>
+void launch_fc(FcArgs a, hipStream_t s) {
+  a.mt = (a.M + WM * FM * 16 - 1) / (WM * FM * 16);
+  a.nt = (a.N + WN * FN * 16 - 1) / (WN * FN * 16);
+  hipLaunchKernelGGL((fc_i8<T, WM, WN, FM, FN>), dim3((unsigned)(a.mt * a.nt)), dim3(64 * WM * WN), 0, s, a);
+}
+
+int64_t tiles(const FcArgs &a, int64_t b) { return ((a.M + b - 1) / b) * ((a.N + b - 1) / b); }
+
+template <typename T>
+lpg_status run_fc(const FcArgs &a, hipStream_t s) {
+  // the largest tile that still gives most CUs a block
+  if (tiles(a, 256) >= 192) launch_fc<T, 2, 4, 8, 4>(a, s);
+  else if (tiles(a, 128) >= 192) launch_fc<T, 2, 2, 4, 4>(a, s);
+  else launch_fc<T, 2, 2, 2, 2>(a, s);
+  LPG_HIP(hipGetLastError());
+  return LPG_OK;
+}
+
+template <typename T>
+lpg_status run_rows(const RowsArgs &a, hipStream_t s) {
+  const int kp = (a.K1 + a.K2 + 1023) / 1024 * 1024;
+  const dim3 g((unsigned)((a.N + 3) / 4)), b(256);
+  if (a.M == 1) hipLaunchKernelGGL((fc_i8_rows<T, 1>), g, b, kp, s, a);
+  else if (a.M == 2) hipLaunchKernelGGL((fc_i8_rows<T, 2>), g, b, 2 * kp, s, a);
+  else if (a.M <= 4) hipLaunchKernelGGL((fc_i8_rows<T, 4>), g, b, a.M * kp, s, a);
+  else hipLaunchKernelGGL((fc_i8_rows<T, kRows>), g, b, a.M * kp, s, a);
+  LPG_HIP(hipGetLastError());
+  return LPG_OK;
+}
+
+constexpr int64_t kMaxK = 131072;  // 131072 * 127^2 < 2^31
+
+}  // namespace
+}  // namespace lpg
+
+using namespace lpg;
+
+#define LPG_I8_TYPES(what, f)                                                            \
+  do {                                                                                   \
+    if (dtype == LPG_F32) return f(float);                                               \
+    if (dtype == LPG_BF16) return f(__bf16);                                             \
+    if (dtype == LPG_F16) return f(_Float16);                                            \
+    ::lpg::set_error(what ": dtype %d (LPG_BF16, LPG_F16 or LPG_F32)", (int)dtype);      \
+    return LPG_ERR_INVALID;                                                              \
+  } while (0)
+
+extern "C" lpg_status lpg_quant_i8(int32_t dtype, int64_t M, int64_t K1, const void *x, int64_t ldx, int64_t K2,
+                                   const void *x2, int64_t ldx2, int8_t *q, int64_t ldq, float *scale, void *stream) {
+  LPG_REQUIRE(M >= 0 && K1 >= 1 && K2 >= 0 && K1 <= kMaxK && K2 <= kMaxK && K1 + K2 <= kMaxK,
+              "lpg_quant_i8: need M >= 0, K1 >= 1, K2 >= 0, K1 + K2 <= 131072");
+  LPG_REQUIRE(ldx >= K1 && (K2 == 0 || ldx2 >= K2), "lpg_quant_i8: row strides below the columns");
+  LPG_REQUIRE(ldq >= K1 + K2 && ldq % 128 == 0, "lpg_quant_i8: ldq must be a multiple of 128 that holds K1 + K2");
+  LPG_REQUIRE(M == 0 || (x && q && scale && (K2 == 0 || x2)), "lpg_quant_i8: NULL pointer");
+  LPG_REQUIRE(aligned16(q), "lpg_quant_i8: q must be 16-byte aligned");
+  LPG_REQUIRE((M + 3) / 4 <= INT32_MAX, "lpg_quant_i8: too many rows");
+  const QuantArgs a{M, ldx, ldx2, ldq, (int)K1, (int)K2, x, x2, q, scale};
+  const auto go = [&](auto kernel) -> lpg_status {
+    if (M == 0) return LPG_OK;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((M + 3) / 4)), dim3(256), 0, as_stream(stream), a);
+    LPG_HIP(hipGetLastError());
+    return LPG_OK;
+  };
+#define F(T) go(quant_rows<T>)
+  LPG_I8_TYPES("lpg_quant_i8", F);
+#undef F
+}
+
+extern "C" lpg_status lpg_fc_i8(int32_t dtype, int64_t M, int64_t N, int64_t K, const int8_t *q, int64_t ldq,
+                                const float *scale, const int8_t *w, int64_t ldw, const float *wscale, const float *bias,
+                                int32_t flags, void *y, int64_t ldy, void *stream) {
+  LPG_REQUIRE(M >= 0 && N >= 1 && K >= 1 && K <= kMaxK, "lpg_fc_i8: need M >= 0, N >= 1, 1 <= K <= 131072");
+  LPG_REQUIRE(ldq >= K && ldq % 128 == 0 && ldq <= kMaxK, "lpg_fc_i8: ldq must be a multiple of 128 that holds K");
+  LPG_REQUIRE(ldw % 16 == 0 && ldw >= (K + 15) / 16 * 16 && ldw <= (int64_t)1 << 22,
+              "lpg_fc_i8: ldw must be a multiple of 16 that holds K, at most 2^22");
+  LPG_REQUIRE(ldy >= N && (flags & ~LPG_FC_RELU) == 0, "lpg_fc_i8: ldy below N or unknown flags");
+  LPG_REQUIRE(w && wscale && (M == 0 || (q && scale && y)), "lpg_fc_i8: NULL pointer");
+  LPG_REQUIRE(aligned16(q) && aligned16(w), "lpg_fc_i8: q and w must be 16-byte aligned");
+  LPG_REQUIRE(((M + 63) / 64) <= INT32_MAX / ((N + 63) / 64), "lpg_fc_i8: too many tiles");
+  const FcArgs a{M, N, ldq, ldw, ldy, (int)K, q, w, scale, wscale, bias, y, 0, 0, (flags & LPG_FC_RELU) ? 1 : 0};
+#define F(T) M == 0 ? LPG_OK : run_fc<T>(a, as_stream(stream))
+  LPG_I8_TYPES("lpg_fc_i8", F);
+#undef F
+}
+
+extern "C" lpg_status lpg_fc_i8_rows(int32_t dtype, int64_t M, int64_t N, int64_t K1, const void *x, int64_t ldx,
+                                     int64_t K2, const void *x2, int64_t ldx2, const int8_t *w, int64_t ldw,
+                                     const float *wscale, const float *bias, int32_t flags, void *y, int64_t ldy,
+                                     void *stream) {
+  LPG_REQUIRE(M >= 0 && M <= kRows && N >= 1 && N <= INT32_MAX && K1 >= 1 && K2 >= 0 && K1 <= kMaxK && K2 <= kMaxK,
+              "lpg_fc_i8_rows: need 0 <= M <= 8, N >= 1, K1 >= 1, K2 >= 0");
+  const int64_t K = K1 + K2;
+  if ((K + 1023) / 1024 * 1024 * (M < 1 ? 1 : M) > kRowsBytes) {
+    set_error("lpg_fc_i8_rows: the rows' codes take more than %d bytes (use lpg_quant_i8 and lpg_fc_i8)", kRowsBytes);
+    return LPG_ERR_UNSUPPORTED;
+  }
+  LPG_REQUIRE(ldx >= K1 && (K2 == 0 || ldx2 >= K2) && ldy >= N, "lpg_fc_i8_rows: row strides below the columns");
+  LPG_REQUIRE(ldw % 16 == 0 && ldw >= (K + 15) / 16 * 16, "lpg_fc_i8_rows: ldw must be a multiple of 16 that holds K");
+  LPG_REQUIRE((flags & ~LPG_FC_RELU) == 0, "lpg_fc_i8_rows: unknown flags");
+  LPG_REQUIRE(w && wscale && (M == 0 || (x && y && (K2 == 0 || x2))), "lpg_fc_i8_rows: NULL pointer");
+  LPG_REQUIRE(aligned16(w), "lpg_fc_i8_rows: w must be 16-byte aligned");
+  const RowsArgs a{N,  ldx, ldx2, ldw,    ldy,  (int)M, (int)K1, (int)K2,
+                   x,  x2,  w,    wscale, bias, y,      (flags & LPG_FC_RELU) ? 1 : 0};
+#define F(T) M == 0 ? LPG_OK : run_rows<T>(a, as_stream(stream))
+  LPG_I8_TYPES("lpg_fc_i8_rows", F);
+#undef F
+}

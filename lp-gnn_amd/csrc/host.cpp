@@ -42,6 +42,9 @@ struct Lib {
   decltype(&lpg_adamw8) adamw8 = nullptr;
   decltype(&lpg_grad_norm_workspace_bytes) grad_norm_workspace_bytes = nullptr;
   decltype(&lpg_grad_norm) grad_norm = nullptr;
+  decltype(&lpg_quant_i8) quant_i8 = nullptr;
+  decltype(&lpg_fc_i8) fc_i8 = nullptr;
+  decltype(&lpg_fc_i8_rows) fc_i8_rows = nullptr;
 } L;
 
 void open(const std::string &path) {
@@ -58,6 +61,9 @@ void open(const std::string &path) {
   SYM(adamw8);
   SYM(grad_norm_workspace_bytes);
   SYM(grad_norm);
+  SYM(quant_i8);
+  SYM(fc_i8);
+  SYM(fc_i8_rows);
 #undef SYM
 }
 
@@ -78,10 +84,13 @@ int32_t code_of(at::ScalarType t) {
   return t == at::kBFloat16 ? LPG_BF16 : t == at::kHalf ? LPG_F16 : t == at::kFloat ? LPG_F32 : -1;
 }
 
+// the row stride of a matrix (that of a single row says nothing)
+int64_t ld(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
 // t as [rows, D] with contiguous rows (a copy only where its strides allow no view)
 Tensor rows(const Tensor &t) {
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
-  return r.stride(1) == 1 && r.stride(0) >= r.size(1) ? r : r.contiguous();
+  return (r.stride(1) == 1 || r.size(1) == 1) && ld(r) >= r.size(1) ? r : r.contiguous();
 }
 
 // ------------------------------------------------------------------ layer norm
@@ -95,7 +104,7 @@ Tensor norm_forward(const Tensor &x, const Tensor &w, const Tensor &b, double ep
   Tensor y = at::empty({M, D}, x.options());
   if (stats) *stats = at::empty({2, M}, x.options().dtype(at::kFloat));
   float *mean = stats ? stats->data_ptr<float>() : nullptr;
-  check(L.layer_norm_fwd(code_of(x.scalar_type()), weight_code(w, b), M, D, x.data_ptr(), x.stride(0), ptr(w), ptr(b),
+  check(L.layer_norm_fwd(code_of(x.scalar_type()), weight_code(w, b), M, D, x.data_ptr(), ld(x), ptr(w), ptr(b),
                          (float)eps, relu ? LPG_NORM_RELU : 0, y.data_ptr(), D, mean, mean ? mean + M : nullptr,
                          stream_of(x)),
         "lpg_layer_norm_fwd");
@@ -130,8 +139,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     if (dw.defined() || db.defined())
       ws = at::empty({L.layer_norm_bwd_workspace_bytes(M, D) / 4}, x.options().dtype(at::kFloat));
     const float *mean = stats.data_ptr<float>();
-    check(L.layer_norm_bwd(code_of(x.scalar_type()), weight_code(w, b), M, D, x.data_ptr(), x.stride(0), dy.data_ptr(),
-                           dy.stride(0), ptr(w), ptr(b), mean, mean + M,
+    check(L.layer_norm_bwd(code_of(x.scalar_type()), weight_code(w, b), M, D, x.data_ptr(), ld(x), dy.data_ptr(),
+                           ld(dy), ptr(w), ptr(b), mean, mean + M,
                            ctx->saved_data["relu"].toBool() ? LPG_NORM_RELU : 0, ptr(dx), D, ptr(dw), ptr(db), ptr(ws),
                            stream_of(x)),
           "lpg_layer_norm_bwd");
@@ -215,6 +224,12 @@ const float *scale_ptr(const char *what, const OptTensor &s, const Tensors &ps) 
   return s->data_ptr<float>();
 }
 
+// the kernels write through pointers: tell autograd (and whatever keeps values by version), as an in-place op
+void written(const Tensors &ts) {
+  for (const Tensor &t : ts)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void adamw_step(const Tensors &ps, const Tensors &gs, const Tensors &ms, const Tensors &vs, int64_t step, double lr,
                 std::pair<double, double> betas, double eps, double weight_decay, const OptTensor &grad_scale) {
   const char *what = "adamw_step";
@@ -231,6 +246,7 @@ void adamw_step(const Tensors &ps, const Tensors &gs, const Tensors &ms, const T
     tab[i] = {ps[i].data_ptr(), gs[i].data_ptr(), ptr_of<float>(ms[i]), ptr_of<float>(vs[i]), ps[i].numel()};
   const c10::DeviceGuard guard(ps[0].device());
   check(L.adamw(type, (int64_t)tab.size(), tab.data(), &h, scale, stream_of(ps[0])), "lpg_adamw");
+  written(ps), written(ms), written(vs);
 }
 
 // The 32-bit integer hash of the kernels' random bits (fc_common.h lowbias32), for the rounding key of a
@@ -272,6 +288,7 @@ void adamw_step_8bit(const Tensors &ps, const Tensors &gs, const Tensors &m8, co
               r8[i].data_ptr(), ptr_of<float>(rs[i]), ps[i].numel(),    rounding_key(places ? (*places)[i] : (int64_t)i, step, seed)};
   const c10::DeviceGuard guard(ps[0].device());
   check(L.adamw8(type, (int64_t)tab.size(), tab.data(), &h, scale, stream_of(ps[0])), "lpg_adamw8");
+  written(ps), written(m8), written(ms), written(r8), written(rs);
 }
 
 std::pair<Tensor, Tensor> clip_scale(const Tensors &gs, double max_norm) {
@@ -291,6 +308,88 @@ std::pair<Tensor, Tensor> clip_scale(const Tensors &gs, double max_norm) {
   return {out[0], out[1]};
 }
 
+// ------------------------------------------------------------------ 8-bit integers
+// x [.., K1] (and x2 [.., K2], the same rows) as row matrices
+std::pair<Tensor, Tensor> i8_rows(const char *what, const Tensor &x, const OptTensor &x2) {
+  REQUIRE(x.is_cuda(), "lpgnn ", what, ": runs on a HIP device only (no CPU path)");
+  REQUIRE(code_of(x.scalar_type()) >= 0, "lpgnn ", what, ": x must be float32, bfloat16 or float16, got ",
+          x.scalar_type());
+  REQUIRE(x.dim() > 0 && x.size(-1) > 0, "lpgnn ", what, ": x needs columns, got shape ", x.sizes());
+  REQUIRE(!at::GradMode::is_enabled() || !(x.requires_grad() || (x2 && x2->requires_grad())), "lpgnn ", what,
+          ": 8-bit integers have no gradient (call it under torch.no_grad())");
+  if (!x2) return {rows(x), Tensor()};
+  REQUIRE(x2->device() == x.device() && x2->scalar_type() == x.scalar_type() && x2->dim() == x.dim() &&
+              x2->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1) && x2->size(-1) > 0,
+          "lpgnn ", what, ": x2 must have x's rows, type and device, got ", x2->sizes(), " ", x2->scalar_type(), " beside ",
+          x.sizes(), " ", x.scalar_type());
+  return {rows(x), rows(*x2)};
+}
+
+std::pair<Tensor, Tensor> quant(const Tensor &x, const Tensor &x2) {
+  const int64_t M = x.size(0), K1 = x.size(1), K2 = x2.defined() ? x2.size(1) : 0, ldq = (K1 + K2 + 127) / 128 * 128;
+  Tensor q = at::empty({M, ldq}, x.options().dtype(at::kChar)), s = at::empty({M}, x.options().dtype(at::kFloat));
+  check(L.quant_i8(code_of(x.scalar_type()), M, K1, x.data_ptr(), ld(x), K2, ptr(x2), K2 ? ld(x2) : 0,
+                   ptr_of<int8_t>(q), ldq, ptr_of<float>(s), stream_of(x)),
+        "lpg_quant_i8");
+  return {q, s};
+}
+
+std::pair<Tensor, Tensor> quantize_i8(const Tensor &x, const OptTensor &x2) {
+  const auto [a, b] = i8_rows("quantize_i8", x, x2);
+  const c10::DeviceGuard guard(x.device());
+  auto [q, s] = quant(a, b);
+  return {q.narrow(1, 0, a.size(1) + (b.defined() ? b.size(1) : 0)), s};
+}
+
+Tensor linear_i8(const Tensor &x, const Tensor &wq, const Tensor &ws, const OptTensor &bias, const OptTensor &x2,
+                 bool relu) {
+  const char *what = "linear_i8";
+  const auto [a, b] = i8_rows(what, x, x2);
+  const int64_t M = a.size(0), K1 = a.size(1), K2 = b.defined() ? b.size(1) : 0, K = K1 + K2;
+  REQUIRE(wq.dim() == 2 && wq.scalar_type() == at::kChar && wq.device() == x.device() && wq.size(1) == K && wq.size(0) > 0,
+          "lpgnn linear_i8: wq must be int8 [N, ", K, "] on ", x.device(), ", got ", wq.scalar_type(), " ", wq.sizes(),
+          " on ", wq.device());
+  const int64_t N = wq.size(0);
+  const auto vec = [&](const char *name, const Tensor &t) {
+    REQUIRE(t.dim() == 1 && t.size(0) == N && t.scalar_type() == at::kFloat && t.device() == x.device(),
+            "lpgnn linear_i8: ", name, " must be float32 [", N, "] on ", x.device(), ", got ", t.scalar_type(), " ",
+            t.sizes(), " on ", t.device());
+    return t.contiguous();
+  };
+  const Tensor scale = vec("ws", ws), bb = bias ? vec("bias", *bias) : Tensor();
+  const c10::DeviceGuard guard(x.device());
+  // rows of w on 16-byte borders, each readable to the next one (quantize_i8's are); else a copy that is
+  Tensor w = wq;
+  const int64_t k16 = (K + 15) / 16 * 16;
+  int64_t ldw = N > 1 ? w.stride(0) : k16;
+  const bool room = (w.storage_offset() + (N - 1) * ldw + k16) <= (int64_t)w.storage().nbytes();
+  if ((w.stride(1) != 1 && K > 1) || ldw < k16 || ldw % 16 || !room || reinterpret_cast<uintptr_t>(w.data_ptr()) % 16) {
+    w = at::empty({N, k16}, wq.options()).narrow(1, 0, K);
+    w.copy_(wq);
+    ldw = k16;
+  }
+  auto shape = x.sizes().vec();
+  shape.back() = N;
+  Tensor y = at::empty({M, N}, x.options());
+  const int32_t type = code_of(x.scalar_type()), flags = relu ? LPG_FC_RELU : 0;
+  if (M > 0 && M <= 8) {
+    const lpg_status st =
+        L.fc_i8_rows(type, M, N, K1, a.data_ptr(), ld(a), K2, ptr(b), K2 ? ld(b) : 0, ptr_of<int8_t>(w),
+                     ldw, ptr_of<float>(scale), ptr_of<float>(bb), flags, y.data_ptr(), N, stream_of(x));
+    if (st != LPG_ERR_UNSUPPORTED) {  // (else: rows too long for its LDS)
+      check(st, "lpg_fc_i8_rows");
+      return y.view(shape);
+    }
+  }
+  if (M > 0) {
+    const auto [q, s] = quant(a, b);
+    check(L.fc_i8(type, M, N, K, ptr_of<int8_t>(q), q.size(1), ptr_of<float>(s), ptr_of<int8_t>(w), ldw,
+                  ptr_of<float>(scale), ptr_of<float>(bb), flags, y.data_ptr(), N, stream_of(x)),
+          "lpg_fc_i8");
+  }
+  return y.view(shape);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -300,4 +399,6 @@ PYBIND11_MODULE(_host, m) {
   m.def("adamw_step", &adamw_step);
   m.def("adamw_step_8bit", &adamw_step_8bit);
   m.def("clip_scale", &clip_scale);
+  m.def("quantize_i8", &quantize_i8);
+  m.def("linear_i8", &linear_i8);
 }

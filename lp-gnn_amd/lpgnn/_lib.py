@@ -121,6 +121,9 @@ HEADER_SYMBOLS = (
     "lpg_adamw8",
     "lpg_grad_norm_workspace_bytes",
     "lpg_grad_norm",
+    "lpg_quant_i8",
+    "lpg_fc_i8",
+    "lpg_fc_i8_rows",
 )
 
 c_i64, c_i32, c_p = ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p
@@ -366,6 +369,13 @@ def lib() -> ctypes.CDLL:
     L.lpg_grad_norm_workspace_bytes.restype = c_i64
     L.lpg_grad_norm.argtypes = [c_i32, c_i64, c_p, ctypes.c_double, c_p, c_p, c_p, c_p]
     L.lpg_grad_norm.restype = c_i32
+    L.lpg_quant_i8.argtypes = [c_i32, c_i64, c_i64, c_p, c_i64, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_p]
+    L.lpg_quant_i8.restype = c_i32
+    L.lpg_fc_i8.argtypes = [c_i32, c_i64, c_i64, c_i64, c_p, c_i64, c_p, c_p, c_i64, c_p, c_p, c_i32, c_p, c_i64, c_p]
+    L.lpg_fc_i8.restype = c_i32
+    L.lpg_fc_i8_rows.argtypes = [c_i32, c_i64, c_i64, c_i64, c_p, c_i64, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_p, c_i32,
+                                 c_p, c_i64, c_p]
+    L.lpg_fc_i8_rows.restype = c_i32
     _lib = L
     return L
 

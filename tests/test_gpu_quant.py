@@ -1,0 +1,196 @@
+"""lpgnn.linear_i8 and quantize_i8 on the GPU: the codes and the sums are exact and the epilogue is a fixed
+chain of fp32 roundings, so results have to be the restatement's bits (tests/i8_ref.py); and within the
+derived bound of the 64-bit formula."""
+import pytest
+import torch
+
+import i8_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+T = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def _case(M, N, K1, K2, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed * 101 + M * 7 + N * 3 + K1)
+    n = lambda *s: torch.randn(*s, generator=g)
+    x = (n(M, K1) * torch.exp(n(M, 1))).to(dtype)
+    x2 = n(M, K2).to(dtype) if K2 else None
+    W, bias = n(N, K1 + K2) * 0.1, n(N)
+    return x, x2, W, bias
+
+
+def _dev(t):
+    return None if t is None else t.to(DEV)
+
+
+def _check(x, x2, W, bias, relu, w=None):
+    from lpgnn import linear_i8, quantize_i8
+
+    wq, ws = quantize_i8(_dev(W)) if w is None else w
+    y = linear_i8(_dev(x), wq, ws, _dev(bias), x2=_dev(x2), relu=relu)
+    xx = x if x2 is None else torch.cat((x, x2), 1)
+    q, s, top = R.quantize(xx)
+    a, sw = wq.cpu(), ws.cpu()
+    assert y.dtype == x.dtype and y.shape == (x.shape[0], a.shape[0])
+    assert torch.equal(y.cpu(), R.linear(q, s, a, sw, bias, relu, x.dtype))
+    y64 = R.linear64(q, top, a, sw, bias, relu)
+    assert ((y.cpu().double() - y64).abs() <= R.bound(q, top, a, sw, bias, y64, x.dtype)).all()
+    return y
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("K1,K2", [(1, 0), (3, 4), (8, 8), (15, 1), (16, 0), (100, 27), (128, 0), (64, 64), (129, 0),
+                                   (200, 200), (1000, 25), (1024, 1024), (5000, 0)])
+def test_codes(K1, K2, dtype):
+    from lpgnn import quantize_i8
+
+    for M in (1, 5, 130):
+        x, x2, _, _ = _case(M, 1, K1, K2, T[dtype])
+        x[0, 0] = x.abs().max() * 2  # 63.5 of 127: an exact border, decided to the even code
+        if K1 > 1:
+            x[0, 1], x[0, K1 - 1] = x[0, 0] / 2, -x[0, 0] / 2
+        q, s = quantize_i8(_dev(x), _dev(x2))
+        want, sw, _ = R.quantize(x if x2 is None else torch.cat((x, x2), 1))
+        assert torch.equal(q.cpu().double(), want) and torch.equal(s.cpu(), sw)
+        assert q.stride(0) % 128 == 0 and not q.as_strided((M, q.stride(0)), (q.stride(0), 1))[:, K1 + K2:].any()
+
+
+def test_codes_next_to_borders():
+    """fp32 numbers on both sides of every border between two codes, one unit in the last place apart: an fp32
+    quotient would put some on the wrong side."""
+    from lpgnn import quantize_i8
+
+    for top in (1.0, 1.7, 3.1415927, 0.1, 127.0, 253.99998):
+        top = torch.tensor(top)
+        b = ((torch.arange(127).double() + 0.5) / 127 * top.double()).float()
+        lo, hi = torch.nextafter(b, torch.tensor(0.0)), torch.nextafter(b, torch.tensor(1e9))
+        row = torch.cat((top[None], lo, b, hi, -lo, -b, -hi))
+        x = row.repeat(70, 1)
+        x[1:] *= (1 + torch.rand(69, 1, generator=torch.Generator().manual_seed(1)))
+        q, s = quantize_i8(_dev(x))
+        want, sw, _ = R.quantize(x)
+        assert torch.equal(q.cpu().double(), want) and torch.equal(s.cpu(), sw)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 8, 9, 63, 64, 65, 130, 300])
+def test_linear(M, dtype):
+    for k, (N, K1, K2) in enumerate(((1, 40, 0), (17, 16, 16), (64, 128, 0), (65, 100, 29), (128, 127, 130), (333, 200, 200),
+                                     (200, 1024, 1024), (20, 4500, 100))):
+        _check(*_case(M, N, K1, K2, T[dtype]), relu=k % 2 == 0)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(128 * 63 + 1, 384, 300), (128 * 64, 383, 128), (256 * 95 + 3, 512, 260),
+                                   (256 * 96, 511, 385), (256 * 96, 264, 512)])
+def test_linear_large_tiles(M, N, K, dtype):
+    """Shapes of the 128 and 256 tiles, with rows, columns and k that end inside one."""
+    _check(*_case(M, N, K, 0, T[dtype]), relu=False)
+
+
+def test_longest_sum_and_largest_codes():
+    """K at its limit with every product 127 * 127: 2114060288, below 2^31."""
+    K = 131072
+    from lpgnn import linear_i8
+
+    wq = torch.full((16, K), 127, dtype=torch.int8, device=DEV)
+    wq[1] = -127
+    for M in (1, 9):
+        y = linear_i8(torch.ones(M, K, device=DEV), wq, torch.ones(16, device=DEV))
+        want = torch.full((M, 16), float(K * 127 * 127)) * (torch.ones(1) / torch.full((1,), 127.0))
+        want[:, 1] *= -1
+        assert torch.equal(y.cpu(), want)
+    with pytest.raises(RuntimeError, match="131072"):
+        linear_i8(torch.ones(9, K + 16, device=DEV), torch.zeros(16, K + 16, dtype=torch.int8, device=DEV),
+                  torch.ones(16, device=DEV))
+
+
+@pytest.mark.parametrize("M", [3, 40])
+def test_bad_and_empty_rows(M):
+    from lpgnn import linear_i8, quantize_i8
+
+    x, x2, W, bias = _case(M, 50, 70, 30, torch.float32)
+    wq, ws = quantize_i8(_dev(W))
+    clean = linear_i8(_dev(x), wq, ws, _dev(bias), x2=_dev(x2), relu=True)
+    x[0], x2[0] = 0.0, 0.0
+    x[1, 5] = float("nan")
+    x2[2, 29] = float("-inf")
+    y = linear_i8(_dev(x), wq, ws, _dev(bias), x2=_dev(x2), relu=True)
+    assert torch.equal(y[0].cpu(), bias.clamp(min=0)) and y[1].isnan().all() and y[2].isnan().all()
+    assert torch.equal(y[3:], clean[3:])
+    x[0] = 2.0 ** -101  # below what the format of the scale holds: zeros
+    assert torch.equal(linear_i8(_dev(x), wq, ws, _dev(bias), x2=_dev(x2))[0].cpu(), bias)
+    x[0] = 2.0 ** -99
+    _check(x[:1], x2[:1], W, None, False)
+    assert linear_i8(_dev(x)[:0], wq, ws, x2=_dev(x2)[:0]).shape == (0, 50)
+
+
+@pytest.mark.parametrize("M", [2, 50])
+def test_strides_and_layouts(M):
+    """Rows inside wider buffers at odd offsets, transposed inputs, weights off 16-byte borders, weights at the
+    very end of their storage, more dimensions."""
+    from lpgnn import linear_i8, quantize_i8
+
+    x, x2, W, bias = _case(M, 37, 75, 33, torch.bfloat16)
+    wq, ws = quantize_i8(_dev(W))
+    want = linear_i8(_dev(x), wq, ws, _dev(bias), x2=_dev(x2))
+    wide = torch.full((M, 200), float("nan"), dtype=x.dtype, device=DEV)
+    wide[:, 3:78], wide[:, 101:134] = _dev(x), _dev(x2)
+    assert torch.equal(linear_i8(wide[:, 3:78], wq, ws, _dev(bias), x2=wide[:, 101:134]), want)
+    assert torch.equal(linear_i8(_dev(x).t().contiguous().t(), wq, ws, _dev(bias), x2=_dev(x2)), want)
+    tight = torch.empty(37 * 108 + 1, dtype=torch.int8, device=DEV)
+    odd = tight[1:].view(37, 108)
+    odd.copy_(wq)
+    end = torch.zeros(36 * 112 + 108, dtype=torch.int8, device=DEV).as_strided((37, 108), (112, 1))
+    end.copy_(wq)
+    for w in (wq.contiguous(), odd, wq.t().contiguous().t(), end):
+        assert torch.equal(linear_i8(_dev(x), w, ws, _dev(bias), x2=_dev(x2)), want)
+    a, b = _dev(x).view(M // 2, 2, 75), _dev(x2).view(M // 2, 2, 33)
+    assert torch.equal(linear_i8(a, wq, ws, _dev(bias), x2=b).view(M, 37), want)
+    one = _dev(x[:1]).t().contiguous().t()  # a single row whose stride is 1
+    assert torch.equal(linear_i8(one, wq, ws, _dev(bias), x2=_dev(x2[:1])), want[:1])
+
+
+def test_other_stream_and_graph():
+    from lpgnn import linear_i8, quantize_i8
+
+    for M in (4, 100):
+        x, x2, W, bias = (_dev(t) for t in _case(M, 64, 80, 40, torch.float16))
+        wq, ws = quantize_i8(W)
+        want = linear_i8(x, wq, ws, bias, x2=x2)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = linear_i8(x, wq, ws, bias, x2=x2)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(got, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = linear_i8(x, wq, ws, bias, x2=x2)
+        for k in range(3):
+            x.mul_(-0.5)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held, linear_i8(x, wq, ws, bias, x2=x2))
+
+
+def test_refusals():
+    from lpgnn import linear_i8, quantize_i8
+
+    x = torch.randn(4, 32, device=DEV)
+    wq, ws = quantize_i8(torch.randn(8, 32, device=DEV))
+    for args, kw, msg in (((x.double(), wq, ws), {}, "float32, bfloat16 or float16"),
+                          ((x, wq[:, :31], ws), {}, "wq must be"),
+                          ((x, wq.short(), ws), {}, "wq must be"),
+                          ((x, wq.cpu(), ws), {}, "wq must be"),
+                          ((x, wq, ws[:7]), {}, "ws must be"),
+                          ((x, wq, ws, torch.ones(8, device=DEV).half()), {}, "bias must be"),
+                          ((x, wq, ws), dict(x2=x), "wq must be"),
+                          ((x[:, :16], wq, ws), dict(x2=x[:3, :16]), "x2 must have"),
+                          ((x[:, :16], wq, ws), dict(x2=x[:, :16].half()), "x2 must have"),
+                          ((x.clone().requires_grad_(True), wq, ws), {}, "no gradient")):
+        with pytest.raises(RuntimeError, match=msg):
+            linear_i8(*args, **kw)
+    with torch.no_grad():
+        linear_i8(x.clone().requires_grad_(True), wq, ws)
