@@ -14,6 +14,10 @@ What runs where:
   heads        lin_left/lin_right -> the same kernel (N = 3 tile)
   add_knowledge                   -> lpg_knowledge_f32 (bitwise torch-CPU
                                      F.normalize semantics)
+  norm="layer" (not in the        -> lpgnn.norm (layer norm + ReLU behind every
+  reference)                         layer of each side)
+  quantize_int8() (evaluation)    -> lpgnn.quant (the hidden layers' FC in 8-bit
+                                     integers)
 """
 from __future__ import annotations
 
@@ -28,6 +32,7 @@ from torch import Tensor, nn
 from .sparse import BipartiteCSR, spmm
 from . import conv as _conv
 from . import fc as _fc
+from .norm import LayerNorm
 from .options import DEFAULT as _DEFAULT_OPTIONS, PathOptions
 
 
@@ -154,8 +159,13 @@ class GCN_FC(GCNBase):
     """arch.py:167-193."""
 
     def __init__(self, p, q, hids=128, depth=3, dp=.1, *args, compute_dtype=torch.float32,
-                 options: PathOptions | None = None, **kwargs):
+                 options: PathOptions | None = None, norm: str | None = None, **kwargs):
+        """``norm="layer"``: a layer norm behind every GraphConvTwoDirection, one per side, before its ReLU
+        (hidden layers: conv -> norm -> ReLU -> dropout); its parameters are ``norms.<layer>.<side>.weight`` /
+        ``.bias``.  The reference has none (the default: its state_dict)."""
         super().__init__()
+        if norm not in (None, "none", "layer"):
+            raise ValueError(f"GCN_FC: norm must be None or 'layer', got {norm!r}")
         # the kernel / fusion choices of this model's hot path (lpgnn.options; defaults from the environment)
         self.options = options or _DEFAULT_OPTIONS
         # bf16 = the c5 configuration (BASELINE.json configs[4]): activations,
@@ -173,6 +183,22 @@ class GCN_FC(GCNBase):
         self.lin_left = nn.Linear(hids, 3)
         self.lin_right = nn.Linear(hids, 3)
         self.dp = dp
+        if norm == "layer":
+            self.norms = nn.ModuleList(nn.ModuleDict(dict(left=LayerNorm(hids), right=LayerNorm(hids)))
+                                       for _ in range(depth - 1))
+        else:
+            self.norms = None
+        self._int8 = None
+
+    def quantize_int8(self, on: bool = True) -> "GCN_FC":
+        """Evaluation in 8-bit integers from here on: the weights of the hidden layers' fully connected parts
+        are quantised now (one scale an output channel), their inputs row by row in every forward
+        (lpgnn.quant.linear_i8); conv1 (8 + 8 columns), the SpMMs, norms and heads keep their type.  Call it
+        again after the weights change (a forward with other weights raises); ``on=False`` goes back."""
+        self._int8 = None
+        if on:
+            self._int8 = [_conv.quantize_two_direction(c.left2right, c.right2left) for c in self.layers]
+        return self
 
     def set_compute_dtype(self, dtype) -> "GCN_FC":
         """fp32 (default) or bf16 activations / SpMM / MFMA FC (fp32 master
@@ -199,6 +225,13 @@ class GCN_FC(GCNBase):
                 raise RuntimeError("GCN_FC: fp16 is the reference's inference mode (val.py:269 model.half() "
                                    "+ model.eval()); train in fp32 or bf16")
             cd = torch.float16
+        if self.norms is not None or (self._int8 is not None and not self.training):
+            left, right = self._normed_or_int8(x_left.to(cd), x_right.to(cd), edge_index)
+            left = _fc.linear(left, self.lin_left.weight, self.lin_left.bias, opts=self.options)
+            right = _fc.linear(right, self.lin_right.weight, self.lin_right.bias, opts=self.options)
+            if not half:
+                left, right = left.float(), right.float()
+            return add_knowledge(left, right, x_left, x_right)
         # conv -> ReLU (arch.py:181-182): the ReLU is the FC kernel's epilogue.
         opts = self.options
         dp = self.dp if self.training else 0.0
@@ -244,6 +277,25 @@ class GCN_FC(GCNBase):
         if half:  # arch.py:191 on the fp16 logits, in half precision (fp16 out, as the reference's)
             return add_knowledge(left, right, x_left, x_right)
         return add_knowledge(left.float(), right.float(), x_left, x_right)
+
+    def _normed_or_int8(self, left, right, edge_index):
+        """The layers with a norm behind each (conv -> norm + ReLU in one pass -> dropout) and / or with 8-bit
+        hidden layers: no fold across layers (a norm lies between them, or no gradient is wanted)."""
+        if not isinstance(edge_index, BipartiteCSR) or getattr(edge_index, "partitioned_conv", None) is not None:
+            raise RuntimeError("GCN_FC: norm='layer' and quantize_int8() run on whole graphs only, not on a "
+                               "row-partitioned adjacency")
+        opts, normed = self.options, self.norms is not None
+        for k, conv in enumerate([self.conv1, *self.layers]):
+            drop = self.dp if self.training and k > 0 else 0.0
+            if k > 0 and self._int8 is not None and not self.training:
+                left, right = _conv.two_direction_i8(left, right, edge_index, self._int8[k - 1], not normed, opts)
+            else:
+                left, right = conv(left, right, edge_index, relu=not normed, dropout=0.0 if normed else drop, opts=opts)
+            if normed:
+                left, right = self.norms[k]["left"](left, relu=True), self.norms[k]["right"](right, relu=True)
+                if drop > 0:
+                    left, right = F.dropout(left, drop), F.dropout(right, drop)
+        return left, right
 
 
 _ARCH_RE = re.compile(r"^\s*([A-Za-z_]\w*)\s*\((.*)\)\s*$", re.S)

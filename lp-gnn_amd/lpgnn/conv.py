@@ -42,6 +42,7 @@ from torch import Tensor
 
 from . import fc as _fc
 from .options import DEFAULT, PathOptions
+from .quant import linear_i8, quantize_i8
 from .sparse import BipartiteCSR, CSR, spmm_forward as _spmm_forward
 
 _GEMM_FLOPS = 160e12  # in-step rates used only to pick the cheaper association
@@ -471,3 +472,33 @@ def two_direction(left: Tensor, right: Tensor, adj: BipartiteCSR, left2right, ri
                                left2right.lin_root.weight, right2left.lin_rel.weight, right2left.lin_rel.bias,
                                right2left.lin_root.weight, bool(relu), float(dropout), prev, opts,
                                bool(feeds_conv and torch.is_grad_enabled()))
+
+
+def quantize_two_direction(left2right, right2left):
+    """The 8-bit weights of a layer's two directions, for two_direction_i8: per direction the codes and channel
+    scales of [W_rel | W_root], the fp32 bias, and what the parameters were (to notice that they changed)."""
+    out = []
+    for d in (left2right, right2left):
+        ts = [d.lin_rel.weight, d.lin_root.weight] + ([] if d.lin_rel.bias is None else [d.lin_rel.bias])
+        with torch.no_grad():
+            wq, ws = quantize_i8(ts[0].detach(), ts[1].detach())
+            bias = None if d.lin_rel.bias is None else d.lin_rel.bias.detach().float().clone()
+        out.append((wq, ws, bias, [(t, t.data_ptr(), None if t.is_inference() else t._version) for t in ts], d))
+    return out
+
+
+def two_direction_i8(left: Tensor, right: Tensor, adj: BipartiteCSR, layer, relu: bool, opts: PathOptions = DEFAULT):
+    """GraphConvTwoDirection.forward (arch.py:65-81) for evaluation with the layer's 8-bit weights
+    (quantize_two_direction): the SpMMs in the activations' type, lin_rel + lin_root + bias (+ ReLU) of each
+    direction one linear_i8 over [aggregate | own features]."""
+    def direction(S, x_src, x_dst, q):
+        wq, ws, bias, seen, d = q
+        now = [d.lin_rel.weight, d.lin_root.weight] + ([] if d.lin_rel.bias is None else [d.lin_rel.bias])
+        for t, (was, at, version) in zip(now, seen):
+            if t is not was or t.data_ptr() != at or (version is not None and t._version != version):
+                raise RuntimeError("GCN_FC: the weights changed since quantize_int8(); call it again")
+        return linear_i8(_spmm_forward(S, x_src, heavy=opts.spmm_heavy), wq, ws, bias, x2=x_dst, relu=relu)
+
+    if torch.is_grad_enabled() and (left.requires_grad or right.requires_grad):
+        raise RuntimeError("GCN_FC: 8-bit evaluation has no gradient (call the model under torch.no_grad())")
+    return direction(adj.fwd, right, left, layer[1]), direction(adj.bwd, left, right, layer[0])

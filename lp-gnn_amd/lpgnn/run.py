@@ -27,6 +27,10 @@ What is different, and why:
   model), and every evaluated batch goes through ``batch_to(half=True)``
   (val.py:31): the fp16 kernels (fp16 storage, fp32 accumulation).  Training
   stays fp32 with the flag set;
+* beyond the reference: ``--opt adamw`` / ``adamw8`` (lpgnn.optim.AdamW, moments in
+  32 or 8 bits) with ``--max_grad_norm``; ``--arch "GCN_FC(..., norm='layer')"`` (a layer
+  norm behind every layer); ``--int8 1``: the VALIDATION model's hidden layers in 8-bit
+  integers (with or without ``--fp16``; whole graphs only);
 * ``--replicas`` (torch.distributed initialised, world > 1): data parallel
   over graphs ("many small LPs: replicas only").  Every rank
   walks the same shuffled epoch order and takes every world-th graph; the
@@ -218,6 +222,10 @@ def parser():
     ap.add_argument("--split", type=str, default="val")
     ap.add_argument("--log_prefix", type=str, default=os.path.abspath("./runs/"))
     ap.add_argument("--fp16", type=int, default=0)
+    ap.add_argument("--int8", type=int, default=0,
+                    help="val: the hidden layers in 8-bit integers (GCN_FC.quantize_int8)")
+    ap.add_argument("--max_grad_norm", type=float, default=0.0,
+                    help="--opt adamw / adamw8: clip the gradients' global norm (0 = off)")
     ap.add_argument("--prefetch_factor", type=int, default=2)
     ap.add_argument("--replicas", type=int, default=0,
                     help="data parallel over graphs when torch.distributed is initialised (world > 1)")
@@ -262,7 +270,10 @@ def make_model(args, for_eval: bool = False):
         model.load(args.load_from)
     if args.fp16 and for_eval:
         model.half()
-    return model.to(args.dev)
+    model = model.to(args.dev)
+    if getattr(args, "int8", 0) and for_eval:
+        model.quantize_int8()
+    return model
 
 
 def _dist_world():
@@ -319,7 +330,8 @@ def run_exp(args, model=None, ds=None):
         ds = LPDataset(args.dataset_processed_prefix, thresh_num=args.edge_num_thresh, device=args.dev)
     train_ds, _ = split_train_val(ds, args.seed)
     model = make_model(args) if model is None else model.to(args.dev)
-    opt, scheduler = make_optimizer(model, args.opt, args.lr, args.epochs)
+    opt, scheduler = make_optimizer(model, args.opt, args.lr, args.epochs,
+                                    getattr(args, "max_grad_norm", 0.0) or None)
     loss_fn = LOSSES[args.loss] if args.loss in LOSSES else None
     if loss_fn is None:
         raise ValueError(f"unknown --loss {args.loss!r} (train.py: balanced / unbalanced / focal)")

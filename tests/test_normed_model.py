@@ -1,0 +1,51 @@
+"""GCN_FC(norm="layer"), the AdamW choices and 8-bit evaluation: construction and refusals on the CPU."""
+import pytest
+import torch
+
+
+def test_default_model_is_unchanged():
+    from lpgnn import GCN_FC
+
+    torch.manual_seed(0)
+    a = GCN_FC(8, 8, hids=32, depth=4)
+    torch.manual_seed(0)
+    b = GCN_FC(8, 8, hids=32, depth=4, norm="layer")
+    assert not any(k.startswith("norms") for k in a.state_dict())
+    for k, v in a.state_dict().items():
+        assert torch.equal(v, b.state_dict()[k])  # the norms draw no random numbers
+    extra = set(b.state_dict()) - set(a.state_dict())
+    assert extra == {f"norms.{i}.{s}.{p}" for i in range(3) for s in ("left", "right") for p in ("weight", "bias")}
+
+
+def test_arch_string_and_refusals():
+    from lpgnn import GCN_FC, build_model
+
+    m = build_model("GCN_FC(8,8,hids=16,depth=3,norm='layer')")
+    assert len(m.norms) == 2 and m.norms[0]["left"].dim == 16
+    assert build_model("GCN_FC(8,8,hids=16,depth=3,norm=None)").norms is None
+    with pytest.raises(ValueError, match="norm"):
+        GCN_FC(8, 8, norm="batch")
+
+
+def test_make_optimizer_choices():
+    from lpgnn import GCN_FC, optim
+    from lpgnn.train import make_optimizer
+
+    m = GCN_FC(8, 8, hids=16)
+    o, s = make_optimizer(m, "adamw", 1e-3, 8, max_grad_norm=2.0)
+    assert isinstance(o, optim.AdamW) and o.state_bits == 32 and o.max_grad_norm == 2.0
+    assert o.param_groups[0]["weight_decay"] == 1e-2 and s.step_size == 2
+    assert make_optimizer(m, "adamw8")[0].state_bits == 8
+    assert type(make_optimizer(m, "adam")[0]) is torch.optim.Adam
+    assert type(make_optimizer(m, "sgd")[0]) is torch.optim.SGD
+    with pytest.raises(ValueError, match="max_grad_norm"):
+        make_optimizer(m, "adam", max_grad_norm=1.0)
+
+
+def test_cli_flags():
+    from lpgnn import run
+
+    a = run.parse_args(["train", "--opt", "adamw8", "--max_grad_norm", "0.5", "--int8", "1"])
+    assert a.opt == "adamw8" and a.max_grad_norm == 0.5 and a.int8 == 1
+    b = run.parse_args([])
+    assert b.max_grad_norm == 0 and b.int8 == 0
