@@ -170,27 +170,27 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   return max(b[0], b[1]);
 }
 
-struct Scale8 {
-  float inv, scale;
-  bool live;
-  // of the block whose largest |x| has these bits; below 1e-30 the block is zero (448 / largest would overflow)
-  __device__ __forceinline__ explicit Scale8(uint32_t top_bits) {
-    const float top = __uint_as_float(top_bits);
-    const bool bad = top_bits >= 0x7f800000u;
-    live = !bad && top >= 1e-30f;
-    inv = live ? 448.f / top : 0.f;
-    scale = bad ? __uint_as_float(0x7fc00000u) : (live ? top / 448.f : 0.f);
+// The scales of a block's two moments, from the bits of their largest |x|, by one division of the wave: its
+// lower half divides for m, its upper for r.  inv = 448 / largest takes the block to the format's range (below
+// 1e-30 the block is zero: 448 / largest would overflow), scale = largest / 448 back.
+struct Scales8 {
+  float inv_m, inv_r, scale_m, scale_r;
+  __device__ __forceinline__ Scales8(uint32_t mt, uint32_t rt, int lane) {
+    const auto norm = [](uint32_t bits) { return bits < 0x7f800000u && __uint_as_float(bits) >= 1e-30f; };
+    const bool lm = norm(mt), lr = norm(rt);
+    // quarters of the wave: 448 / m, m / 448, 448 / r, r / 448
+    const float top = __uint_as_float(lane < 32 ? mt : rt);
+    const float v = lane & 16 ? top / 448.f : 448.f / top;
+    const auto at = [&](int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l)); };
+    const auto scale = [&](uint32_t bits, bool live, int l) {
+      return bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : (live ? at(l) : 0.f);
+    };
+    inv_m = lm ? at(0) : 0.f;
+    inv_r = lr ? at(32) : 0.f;
+    scale_m = scale(mt, lm, 16);
+    scale_r = scale(rt, lr, 48);
   }
 };
-
-// |x| as an e4m3 code without its sign, the 16 random bits u added below the kept mantissa.  Below 2^-6
-// the format steps by 2^-9: adding 2^-6 puts those steps where the kept bits end.
-__device__ __forceinline__ uint32_t to_e4m3(float x, uint32_t u, const Scale8 &s) {
-  const float t = fminf(fabsf(x) * s.inv, 448.f);
-  const bool low = t < 0x1p-6f;
-  const uint32_t bits = __float_as_uint(low ? t + 0x1p-6f : t) + (u << 4);
-  return s.live ? (bits >> 20) - (120u << 3) - (low ? 8u : 0u) : 0u;
-}
 
 template <typename T>
 __global__ __launch_bounds__(kT) void adamw8(Table8 tab) {
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kT) void adamw8(Table8 tab) {
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t q = base / kQ + u * (kT / 64) + wave, i = q * kQ + lane * 4;
-    if (q * kQ >= e.n) continue;  // (the whole wave)
+    if (q * kQ >= e.n) continue;  // (the whole wave: what follows has every lane)
     const int n = e.n - i >= 4 ? 4 : (e.n - i > 0 ? (int)(e.n - i) : 0);
     const auto ma = __builtin_amdgcn_cvt_pk_f32_fp8(mq[u], false), mb = __builtin_amdgcn_cvt_pk_f32_fp8(mq[u], true);
     const auto ra = __builtin_amdgcn_cvt_pk_f32_fp8(rq[u], false), rb = __builtin_amdgcn_cvt_pk_f32_fp8(rq[u], true);
@@ -250,18 +250,24 @@ __global__ __launch_bounds__(kT) void adamw8(Table8 tab) {
         rt = max(rt, __float_as_uint(fabsf(r[j])));
       }
     }
-    const Scale8 sm(wave_max(mt)), sr(wave_max(rt));
+    const Scales8 sc(wave_max(mt), wave_max(rt), lane);
+    // the random rounding is the conversion's own: its seed's upper 20 bits are added below the mantissa it
+    // keeps (in the subnormal range, below the 2^-9 it counts in), here 16 random bits and four zeros
     uint32_t mo = 0, ro = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    const float least = sc.inv_r > 0.f ? 0x1p-9f : 0.f;
+    const auto put = [&](auto jc) {
+      constexpr int j = decltype(jc)::value;
       const uint64_t at = (uint64_t)(i + j);
       const uint32_t bits = lowbias32((uint32_t)at ^ key ^ (uint32_t)(at >> 32) * 0x9e3779b9u);
-      const uint32_t mc = to_e4m3(m[j], bits & 0xffffu, sm);
-      uint32_t rc = to_e4m3(r[j], bits >> 16, sr);
-      if (sr.live && r[j] > 0.f && rc == 0) rc = 1;
-      mo |= (mc | (mc && m[j] < 0.f ? 0x80u : 0u)) << (8 * j);
-      ro |= rc << (8 * j);
-    }
+      const float tm = __builtin_amdgcn_fmed3f(m[j] * sc.inv_m, -448.f, 448.f);
+      const float tr = r[j] > 0.f ? fminf(fmaxf(r[j] * sc.inv_r, least), 448.f) : 0.f;
+      mo = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(tm, (int)(bits << 16), (int)mo, j);
+      ro = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(tr, (int)(bits & 0xffff0000u), (int)ro, j);
+    };
+    put(std::integral_constant<int, 0>());
+    put(std::integral_constant<int, 1>());
+    put(std::integral_constant<int, 2>());
+    put(std::integral_constant<int, 3>());
     if (n == 4) {
       st4(p + i, pp[u]);
       __builtin_memcpy(m8 + i, &mo, 4);
@@ -274,27 +280,25 @@ __global__ __launch_bounds__(kT) void adamw8(Table8 tab) {
       }
     }
     if (lane == 0) {
-      e.ms[q] = sm.scale;
-      e.rs[q] = sr.scale;
+      e.ms[q] = sc.scale_m;
+      e.rs[q] = sc.scale_r;
     }
   }
 }
 
-// the block's sum, in thread 0
+// the block's sum, in thread 0 (one call a kernel)
 __device__ __forceinline__ double block_sum(double v) {
-  __shared__ double red[kT];
-  red[threadIdx.x] = v;
+  __shared__ double red[kT / 64];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  for (int w = kT / 2; w > 0; w >>= 1) {
-    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
-    __syncthreads();
-  }
-  return red[0];
+  return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 template <typename T>
 __global__ __launch_bounds__(kT) void sumsq(TableN tab) {
-  constexpr int U = 8;
+  constexpr int U = kNormChunk / (4 * kT);
   const int k = tensor_of(tab);
   const lpg_tensor &e = tab.t[k];
   const T *g = static_cast<const T *>(e.p);
@@ -305,13 +309,11 @@ __global__ __launch_bounds__(kT) void sumsq(TableN tab) {
     for (int j = 0; j < 4; ++j) s = __builtin_fma((double)f[j], (double)f[j], s);
   };
   if (base + kNormChunk <= e.n) {
-    for (int v = 0; v < kNormChunk / (4 * kT * U); ++v) {
-      float f[U][4];
+    float f[U][4];
 #pragma unroll
-      for (int u = 0; u < U; ++u) ld4(g + base + ((v * U + u) * kT + (int)threadIdx.x) * 4, f[u]);
+    for (int u = 0; u < U; ++u) ld4(g + base + (u * kT + (int)threadIdx.x) * 4, f[u]);
 #pragma unroll
-      for (int u = 0; u < U; ++u) add(f[u]);
-    }
+    for (int u = 0; u < U; ++u) add(f[u]);
   } else {
     for (int64_t i = base + (int)threadIdx.x * 4; i < e.n; i += kT * 4) {
       float f[4];
@@ -326,6 +328,7 @@ __global__ __launch_bounds__(kT) void sumsq(TableN tab) {
 __global__ __launch_bounds__(kT) void norm_scale(int64_t n, const double *__restrict__ part, double max_norm, float *norm,
                                                  float *scale) {
   double s = 0;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < n; i += kT) s += part[i];
   s = block_sum(s);
   if (threadIdx.x == 0) {

@@ -152,6 +152,58 @@ __global__ __launch_bounds__(256) void quant_rows(QuantArgs a) {
   if (lane == 0) a.scale[row] = s.scale;
 }
 
+// The same for rows of at most 64 NV vectors, held in registers: one pass, all loads of a row in flight.
+// Vector i of the row is a vector of x or, from K1 / V on, of x2; the columns that fill no vector are lanes of
+// their own.
+template <typename T, int NV>
+__global__ __launch_bounds__(256) void quant_rows_held(QuantArgs a) {
+  constexpr int V = 16 / sizeof(T);
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.M) return;
+  const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+  const T *x2 = a.K2 ? static_cast<const T *>(a.x2) + row * a.ldx2 : nullptr;
+  int8_t *q = a.q + row * a.ldq;
+  const int n1 = a.K1 / V, n2 = a.K2 / V, r1 = a.K1 % V, r2 = a.K2 % V;
+  u32x4 v[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int i = k * 64 + lane;
+    v[k] = u32x4{0u, 0u, 0u, 0u};
+    if (i < n1 + n2) __builtin_memcpy(&v[k], i < n1 ? x + i * V : x2 + (i - n1) * V, 16);
+  }
+  const float rest[1] = {lane < r1 ? (float)x[n1 * V + lane] : (lane < r1 + r2 ? (float)x2[n2 * V + lane - r1] : 0.f)};
+  uint32_t top = abs_bits(rest[0]);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    T t[V];
+    __builtin_memcpy(t, &v[k], 16);
+#pragma unroll
+    for (int j = 0; j < V; ++j) top = max(top, abs_bits((float)t[j]));
+  }
+  const RowScale s(wave_max(top));
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int i = k * 64 + lane;
+    if (i >= n1 + n2) continue;
+    T t[V];
+    float f[V];
+    uint32_t o[V / 4];
+    __builtin_memcpy(t, &v[k], 16);
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = (float)t[j];
+    quant<V>(f, s, o);
+    __builtin_memcpy(q + (i < n1 ? i * V : a.K1 + (i - n1) * V), o, V);
+  }
+  if (lane < r1 + r2) {
+    uint32_t o[1];
+    quant<1>(rest, s, o);
+    q[lane < r1 ? n1 * V + lane : a.K1 + n2 * V + lane - r1] = (int8_t)o[0];
+  }
+  for (int64_t k = a.K1 + a.K2 + lane; k < a.ldq; k += 64) q[k] = 0;
+  if (lane == 0) a.scale[row] = s.scale;
+}
+
 struct FcArgs {
   int64_t M, N, ldq, ldw, ldy;
   int K;
@@ -499,7 +551,19 @@ extern "C" lpg_status lpg_quant_i8(int32_t dtype, int64_t M, int64_t K1, const v
     LPG_HIP(hipGetLastError());
     return LPG_OK;
   };
-#define F(T) go(quant_rows<T>)
+  // registers for as many vectors as a lane has, up to 16; longer rows are read twice
+  const auto of = [&](auto t) -> lpg_status {
+    using T = decltype(t);
+    constexpr int V = 16 / sizeof(T);
+    const int64_t n = (K1 / V + K2 / V + 63) / 64;
+    if (n <= 1) return go(quant_rows_held<T, 1>);
+    if (n <= 2) return go(quant_rows_held<T, 2>);
+    if (n <= 4) return go(quant_rows_held<T, 4>);
+    if (n <= 8) return go(quant_rows_held<T, 8>);
+    if (n <= 16) return go(quant_rows_held<T, 16>);
+    return go(quant_rows<T>);
+  };
+#define F(T) of(T{})
   LPG_I8_TYPES("lpg_quant_i8", F);
 #undef F
 }

@@ -24,6 +24,8 @@
 // a second kernel adds the partial rows in block order: the same bits every run.
 #include "common.h"
 
+#include <type_traits>
+
 namespace lpg {
 namespace {
 
@@ -39,6 +41,14 @@ template <typename T>
 __device__ __forceinline__ void ldv(const T *p, float (&f)[16 / sizeof(T)]) {
   T t[16 / sizeof(T)];
   __builtin_memcpy(t, p, 16);
+#pragma unroll
+  for (int j = 0; j < (int)(16 / sizeof(T)); ++j) f[j] = (float)t[j];
+}
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ void unpack(u32x4 v, float (&f)[16 / sizeof(T)]) {
+  T t[16 / sizeof(T)];
+  __builtin_memcpy(t, &v, 16);
 #pragma unroll
   for (int j = 0; j < (int)(16 / sizeof(T)); ++j) f[j] = (float)t[j];
 }
@@ -175,7 +185,7 @@ __global__ __launch_bounds__(kT) void norm_fwd(FwdArgs a) {
   }
 }
 
-template <typename T, typename W, int G, int NV>
+template <typename T, typename W, int G, int NV, bool RELU>
 __global__ __launch_bounds__(kT) void norm_bwd(BwdArgs a) {
   constexpr int V = 16 / sizeof(T), R = 64 / G;
   __shared__ float red[2][G * NV * V];
@@ -183,50 +193,77 @@ __global__ __launch_bounds__(kT) void norm_bwd(BwdArgs a) {
   const Cols<G, NV, V> cs(lane % G, (int)a.D);
   float w[NV][V], b[NV][V], dw[NV][V], db[NV][V];
   load_cols<W>(a.w, cs, w, 1.f);
-  load_cols<W>(a.relu ? a.b : nullptr, cs, b, 0.f);
+  if constexpr (RELU) load_cols<W>(a.b, cs, b, 0.f);
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[k][j] = db[k][j] = 0.f;
   const float n = (float)a.D;
   const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy);
-  for (int64_t r0 = ((int64_t)blockIdx.x * kW + wave) * R; r0 < a.M; r0 += (int64_t)gridDim.x * kW * R) {
-    const int64_t row = r0 + slot, at = row < a.M ? row : a.M - 1;
-    const bool in = row < a.M;
+  // the next row's vectors and statistics are loaded while this one is computed
+  u32x4 xn[NV], gn[NV];
+  float mun = 0.f, rsn = 0.f;
+  const int64_t step = (int64_t)gridDim.x * kW * R;
+  const auto fetch = [&](int64_t r0) {
+    const int64_t at = r0 + slot < a.M ? r0 + slot : a.M - 1;
     const T *xr = x + at * a.ldx, *gr = dy + at * a.lddy;
-    float h[NV][V], z[NV][V];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      ldv<T>(xr + cs.c[k], h[k]);
-      ldv<T>(gr + cs.c[k], z[k]);
+      __builtin_memcpy(&xn[k], xr + cs.c[k], 16);
+      __builtin_memcpy(&gn[k], gr + cs.c[k], 16);
     }
-    const float mu = a.mean[at], rs = a.rstd[at];
-    float c1 = 0.f, c2 = 0.f;
+    mun = a.mean[at];
+    rsn = a.rstd[at];
+  };
+  int64_t r0 = ((int64_t)blockIdx.x * kW + wave) * R;
+  if (r0 < a.M) fetch(r0);
+  for (; r0 < a.M; r0 += step) {
+    const int64_t row = r0 + slot;
+    const bool in = row < a.M;
+    u32x4 xc[NV], gc[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) xc[k] = xn[k], gc[k] = gn[k];
+    const float mu = mun, rs = rsn;
+    if (r0 + step < a.M) fetch(r0 + step);
+    // the row stays as it was loaded and h, z are formed twice: of 16-bit rows that is half the registers of
+    // keeping them, and the registers decide how many waves a SIMD holds
+    const auto hz = [&](int k, float (&h)[V], float (&z)[V]) {
+      unpack<T>(xc[k], h);
+      unpack<T>(gc[k], z);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        h[k][j] = (h[k][j] - mu) * rs;
-        if (a.relu && !(__builtin_fmaf(h[k][j], w[k][j], b[k][j]) > 0.f)) z[k][j] = 0.f;
-        if (in && cs.live(k, j)) {
-          dw[k][j] = __builtin_fmaf(z[k][j], h[k][j], dw[k][j]);
-          db[k][j] += z[k][j];
-        }
-        z[k][j] *= w[k][j];
-        if (cs.live(k, j)) {
-          c1 += z[k][j];
-          c2 = __builtin_fmaf(z[k][j], h[k][j], c2);
-        }
+        h[j] = (h[j] - mu) * rs;
+        if constexpr (RELU) z[j] = __builtin_fmaf(h[j], w[k][j], b[k][j]) > 0.f ? z[j] : 0.f;
       }
+    };
+    float c1 = 0.f, c2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float h[V], z[V];
+      hz(k, h, z);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (k == NV - 1) z[j] = cs.live(k, j) ? z[j] : 0.f;
+        const float zi = R > 1 ? (in ? z[j] : 0.f) : z[j];  // (rows past the end: only where a wave has several)
+        dw[k][j] = __builtin_fmaf(zi, h[j], dw[k][j]);
+        db[k][j] += zi;
+        z[j] *= w[k][j];
+        c1 += z[j];
+        c2 = __builtin_fmaf(z[j], h[j], c2);
+      }
+    }
     c1 = row_sum<G>(c1) / n;
     c2 = row_sum<G>(c2) / n;
     if (in && a.dx) {
       T *dr = static_cast<T *>(a.dx) + row * a.lddx;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
+        float h[V], z[V];
+        asm volatile("" : "+v"(xc[k]), "+v"(gc[k]));  // (else the compiler keeps the first pass's h and z)
+        hz(k, h, z);
 #pragma unroll
-        for (int j = 0; j < V; ++j) h[k][j] = __builtin_fmaf(-h[k][j], c2, z[k][j] - c1) * rs;
-        if (k < NV - 1 || cs.lo < V) stv<T>(dr + cs.c[k], h[k]);
+        for (int j = 0; j < V; ++j) h[j] = __builtin_fmaf(-h[j], c2, z[j] * w[k][j] - c1) * rs;
+        if (k < NV - 1 || cs.lo < V) stv<T>(dr + cs.c[k], h);
       }
     }
   }
@@ -354,24 +391,44 @@ __global__ __launch_bounds__(kT) void norm_wgrad_any(BwdArgs a) {
   a.part[(int64_t)blockIdx.y * 2 * a.D + a.D + j] = sb;
 }
 
-// dw, db = the sums of the nblk partial rows [2 D] in block order: 16 columns and 16 row classes a block
-constexpr int kFoldC = 16, kFoldR = kT / kFoldC;
+// dw, db = the sums of the nblk partial rows [2 D]: a block takes 64 columns, a thread four of them and every
+// 64th row (all its loads in flight), the 64 row classes are added by a fixed tree
+constexpr int kFoldC = 64, kFoldT = 1024, kFoldR = kFoldT / (kFoldC / 4);
 template <typename W>
-__global__ __launch_bounds__(kT) void norm_fold(int64_t nblk, int64_t D, const float *__restrict__ part, W *dw, W *db) {
+__global__ __launch_bounds__(kFoldT) void norm_fold(int64_t nblk, int64_t D, const float *__restrict__ part, W *dw, W *db) {
   __shared__ float red[kFoldR][kFoldC];
-  const int c = threadIdx.x % kFoldC, r = threadIdx.x / kFoldC;
-  const int64_t j = (int64_t)blockIdx.x * kFoldC + c;
-  float s = 0.f;
-  if (j < 2 * D)
-    for (int64_t k = r; k < nblk; k += kFoldR) s += part[k * 2 * D + j];
-  red[r][c] = s;
+  const int c = (int)threadIdx.x % (kFoldC / 4) * 4, r = (int)threadIdx.x / (kFoldC / 4);
+  const int64_t j0 = (int64_t)blockIdx.x * kFoldC, j = j0 + c, n = 2 * D - j;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (n >= 4) {
+#pragma unroll 8
+    for (int64_t k = r; k < nblk; k += kFoldR) {
+      float v[4];
+      __builtin_memcpy(v, part + k * 2 * D + j, 16);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s[q] += v[q];
+    }
+  } else if (n > 0) {
+    for (int64_t k = r; k < nblk; k += kFoldR)
+      for (int q = 0; q < 4; ++q) s[q] += q < n ? part[k * 2 * D + j + q] : 0.f;
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) red[r][c + q] = s[q];
   __syncthreads();
-  if (r == 0 && j < 2 * D) {
-    for (int q = 1; q < kFoldR; ++q) s += red[q][c];
-    if (j < D) {
-      if (dw) dw[j] = (W)s;
+  const int col = (int)threadIdx.x % kFoldC, part_of = (int)threadIdx.x / kFoldC;  // 16 parts of 4 classes
+  float t = (red[part_of * 4][col] + red[part_of * 4 + 1][col]) + (red[part_of * 4 + 2][col] + red[part_of * 4 + 3][col]);
+  __syncthreads();
+  red[part_of][col] = t;
+  __syncthreads();
+  if (threadIdx.x < kFoldC && j0 + col < 2 * D) {
+    t = 0.f;
+#pragma unroll
+    for (int q = 0; q < kFoldT / kFoldC; ++q) t += red[q][col];
+    const int64_t at = j0 + col;
+    if (at < D) {
+      if (dw) dw[at] = (W)t;
     } else if (db) {
-      db[j - D] = (W)s;
+      db[at - D] = (W)t;
     }
   }
 }
@@ -440,7 +497,7 @@ lpg_status bwd(BwdArgs a, W *dw, W *db, float *part, hipStream_t s) {
   if (a.M > 0 && in_lanes<T>(a.D)) {
     by_width<T>(a.D, [&](auto g, auto nv) {
       constexpr int G = decltype(g)::value, NV = decltype(nv)::value, R = 64 / G * kW;
-      auto k = norm_bwd<T, W, G, NV>;
+      auto k = a.relu ? norm_bwd<T, W, G, NV, true> : norm_bwd<T, W, G, NV, false>;
       const int64_t most = resident_blocks(k, kT);
       nblk = at_most((a.M + R - 1) / R, most < kPartRows ? most : kPartRows);
       hipLaunchKernelGGL(k, dim3((unsigned)nblk), dim3(kT), 0, s, a);
@@ -459,7 +516,7 @@ lpg_status bwd(BwdArgs a, W *dw, W *db, float *part, hipStream_t s) {
     }
   }
   if (a.part) {  // (no rows: the fold of no partials writes zeros)
-    hipLaunchKernelGGL((norm_fold<W>), dim3((unsigned)((2 * a.D + kFoldC - 1) / kFoldC)), dim3(kT), 0, s, nblk, a.D,
+    hipLaunchKernelGGL((norm_fold<W>), dim3((unsigned)((2 * a.D + kFoldC - 1) / kFoldC)), dim3(kFoldT), 0, s, nblk, a.D,
                        part, dw, db);
     LPG_HIP(hipGetLastError());
   }
