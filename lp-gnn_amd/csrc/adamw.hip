@@ -70,11 +70,24 @@ __device__ __forceinline__ int tensor_of(const Tab &tab) {
   return lo;
 }
 
-// four consecutive elements at any element alignment
+// four consecutive elements at any element alignment, non-temporal
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+  typedef unsigned int words __attribute__((ext_vector_type(4)));
+  typedef unsigned int any __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <>
+struct Four<__bf16> {
+  typedef unsigned int words __attribute__((ext_vector_type(2)));
+  typedef unsigned int any __attribute__((ext_vector_type(2), aligned(2)));
+};
 template <typename T>
 __device__ __forceinline__ void ld4(const T *p, float (&f)[4]) {
+  const typename Four<T>::words w = __builtin_nontemporal_load(reinterpret_cast<const typename Four<T>::any *>(p));
   T t[4];
-  __builtin_memcpy(t, p, sizeof(t));
+  __builtin_memcpy(t, &w, sizeof(t));
 #pragma unroll
   for (int j = 0; j < 4; ++j) f[j] = (float)t[j];
 }
@@ -83,7 +96,9 @@ __device__ __forceinline__ void st4(T *p, const float (&f)[4]) {
   T t[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) t[j] = (T)f[j];
-  __builtin_memcpy(p, t, sizeof(t));
+  typename Four<T>::words w;
+  __builtin_memcpy(&w, t, sizeof(t));
+  __builtin_nontemporal_store(w, reinterpret_cast<typename Four<T>::any *>(p));
 }
 // ... of which `n` (0 to 4) exist; the others read as zero and are not written
 template <typename T>

@@ -36,15 +36,10 @@ __device__ __forceinline__ float to_f(T v) {
   return (float)v;
 }
 
-// 16 bytes from any element-aligned address
-template <typename T>
-__device__ __forceinline__ void ldv(const T *p, float (&f)[16 / sizeof(T)]) {
-  T t[16 / sizeof(T)];
-  __builtin_memcpy(t, p, 16);
-#pragma unroll
-  for (int j = 0; j < (int)(16 / sizeof(T)); ++j) f[j] = (float)t[j];
-}
+// 16 bytes at any element alignment
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
 template <typename T>
 __device__ __forceinline__ void unpack(u32x4 v, float (&f)[16 / sizeof(T)]) {
   T t[16 / sizeof(T)];
@@ -57,7 +52,10 @@ __device__ __forceinline__ void stv(T *p, const float (&f)[16 / sizeof(T)]) {
   T t[16 / sizeof(T)];
 #pragma unroll
   for (int j = 0; j < (int)(16 / sizeof(T)); ++j) t[j] = (T)f[j];
-  __builtin_memcpy(p, t, 16);
+  u32x4 v;
+  __builtin_memcpy(&v, t, 16);
+  if constexpr (sizeof(T) == 2) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_at2 *>(p));
+  else __builtin_nontemporal_store(v, reinterpret_cast<u32x4_at4 *>(p));
 }
 
 template <int CTRL>
@@ -146,11 +144,14 @@ __global__ __launch_bounds__(kT) void norm_fwd(FwdArgs a) {
   T *y = static_cast<T *>(a.y);
   for (int64_t r0 = ((int64_t)blockIdx.x * kW + wave) * R; r0 < a.M; r0 += (int64_t)gridDim.x * kW * R) {
     const int64_t row = r0 + slot;
-    const bool in = row < a.M;
-    const T *xr = x + (in ? row : a.M - 1) * a.ldx;
+    const T *xr = x + (row < a.M ? row : a.M - 1) * a.ldx;
     float f[NV][V];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) ldv<T>(xr + cs.c[k], f[k]);
+    for (int k = 0; k < NV; ++k) {
+      u32x4 raw;
+      __builtin_memcpy(&raw, xr + cs.c[k], 16);
+      unpack<T>(raw, f[k]);
+    }
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(kT) void norm_fwd(FwdArgs a) {
         s = cs.live(k, j) ? __builtin_fmaf(f[k][j], f[k][j], s) : s;
       }
     const float rs = 1.f / sqrtf(row_sum<G>(s) / n + a.eps);
-    if (in) {
+    if (row < a.M) {
       T *yr = y + row * a.ldy;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
@@ -185,9 +186,20 @@ __global__ __launch_bounds__(kT) void norm_fwd(FwdArgs a) {
   }
 }
 
-template <typename T, typename W, int G, int NV, bool RELU>
-__global__ __launch_bounds__(kT) void norm_bwd(BwdArgs a) {
+// U rows a lane group at a time; the next rows' vectors are loaded while these are computed (up to NV = 4: with longer fp32
+// rows the registers hold more by occupancy than by a row ahead).
+// Two waves a SIMD, where the row and its columns' sums leave registers for them (not the longest rows).
+template <typename T, int NV>
+constexpr int bwd_waves() {
+  return NV < (sizeof(T) == 2 ? 4 : 8) ? 2 : 1;
+}
+template <typename T, typename W, int G, int NV, bool RELU, int U>
+__global__ __launch_bounds__(kT, (bwd_waves<T, NV>())) void norm_bwd(BwdArgs a) {
   constexpr int V = 16 / sizeof(T), R = 64 / G;
+  constexpr bool AHEAD = NV <= 4;
+  // h and z of a row are needed twice, for the sums and for dx.  Of 16-bit rows from three vectors on they are
+  // formed twice from the row as it was loaded: half the registers, which decide how many waves a SIMD holds
+  constexpr bool TWICE = sizeof(T) == 2 && NV >= 3;
   __shared__ float red[2][G * NV * V];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slot = lane / G;
   const Cols<G, NV, V> cs(lane % G, (int)a.D);
@@ -200,70 +212,79 @@ __global__ __launch_bounds__(kT) void norm_bwd(BwdArgs a) {
     for (int j = 0; j < V; ++j) dw[k][j] = db[k][j] = 0.f;
   const float n = (float)a.D;
   const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy);
-  // the next row's vectors and statistics are loaded while this one is computed
-  u32x4 xn[NV], gn[NV];
-  float mun = 0.f, rsn = 0.f;
-  const int64_t step = (int64_t)gridDim.x * kW * R;
+  u32x4 xn[U][NV], gn[U][NV];
+  float mun[U], rsn[U];
   const auto fetch = [&](int64_t r0) {
-    const int64_t at = r0 + slot < a.M ? r0 + slot : a.M - 1;
-    const T *xr = x + at * a.ldx, *gr = dy + at * a.lddy;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      __builtin_memcpy(&xn[k], xr + cs.c[k], 16);
-      __builtin_memcpy(&gn[k], gr + cs.c[k], 16);
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = r0 + u * R < a.M ? r0 + u * R : a.M - 1;
+      const T *xr = x + at * a.ldx, *gr = dy + at * a.lddy;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        __builtin_memcpy(&xn[u][k], xr + cs.c[k], 16);
+        __builtin_memcpy(&gn[u][k], gr + cs.c[k], 16);
+      }
+      mun[u] = a.mean[at];
+      rsn[u] = a.rstd[at];
     }
-    mun = a.mean[at];
-    rsn = a.rstd[at];
   };
-  int64_t r0 = ((int64_t)blockIdx.x * kW + wave) * R;
-  if (r0 < a.M) fetch(r0);
-  for (; r0 < a.M; r0 += step) {
-    const int64_t row = r0 + slot;
-    const bool in = row < a.M;
-    u32x4 xc[NV], gc[NV];
+  const int64_t step = (int64_t)gridDim.x * kW * R * U, end = a.M + slot;  // (the waves' loops have no lanes out)
+  int64_t r0 = ((int64_t)blockIdx.x * kW + wave) * R * U + slot;
+  if (AHEAD && r0 < end) fetch(r0);
+  for (; r0 < end; r0 += step) {
+    if (!AHEAD) fetch(r0);
+    u32x4 xc[U][NV], gc[U][NV];
+    float muc[U], rsc[U];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) xc[k] = xn[k], gc[k] = gn[k];
-    const float mu = mun, rs = rsn;
-    if (r0 + step < a.M) fetch(r0 + step);
-    // the row stays as it was loaded and h, z are formed twice: of 16-bit rows that is half the registers of
-    // keeping them, and the registers decide how many waves a SIMD holds
-    const auto hz = [&](int k, float (&h)[V], float (&z)[V]) {
-      unpack<T>(xc[k], h);
-      unpack<T>(gc[k], z);
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        h[j] = (h[j] - mu) * rs;
-        if constexpr (RELU) z[j] = __builtin_fmaf(h[j], w[k][j], b[k][j]) > 0.f ? z[j] : 0.f;
-      }
-    };
-    float c1 = 0.f, c2 = 0.f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      float h[V], z[V];
-      hz(k, h, z);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (k == NV - 1) z[j] = cs.live(k, j) ? z[j] : 0.f;
-        const float zi = R > 1 ? (in ? z[j] : 0.f) : z[j];  // (rows past the end: only where a wave has several)
-        dw[k][j] = __builtin_fmaf(zi, h[j], dw[k][j]);
-        db[k][j] += zi;
-        z[j] *= w[k][j];
-        c1 += z[j];
-        c2 = __builtin_fmaf(z[j], h[j], c2);
-      }
+      for (int k = 0; k < NV; ++k) xc[u][k] = xn[u][k], gc[u][k] = gn[u][k];
+      muc[u] = mun[u], rsc[u] = rsn[u];
     }
-    c1 = row_sum<G>(c1) / n;
-    c2 = row_sum<G>(c2) / n;
-    if (in && a.dx) {
-      T *dr = static_cast<T *>(a.dx) + row * a.lddx;
+    if (AHEAD && r0 + step < end) fetch(r0 + step);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = r0 + u * R;
+      const bool in = row < a.M;
+      const float mu = muc[u], rs = rsc[u];
+      const auto hz = [&](int k, float (&h)[V], float (&z)[V]) {
+        unpack<T>(xc[u][k], h);
+        unpack<T>(gc[u][k], z);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          h[j] = (h[j] - mu) * rs;
+          if constexpr (RELU) z[j] = __builtin_fmaf(h[j], w[k][j], b[k][j]) > 0.f ? z[j] : 0.f;
+        }
+      };
+      float c1 = 0.f, c2 = 0.f;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         float h[V], z[V];
-        asm volatile("" : "+v"(xc[k]), "+v"(gc[k]));  // (else the compiler keeps the first pass's h and z)
         hz(k, h, z);
 #pragma unroll
-        for (int j = 0; j < V; ++j) h[j] = __builtin_fmaf(-h[j], c2, z[j] * w[k][j] - c1) * rs;
-        if (k < NV - 1 || cs.lo < V) stv<T>(dr + cs.c[k], h);
+        for (int j = 0; j < V; ++j) {
+          if (k == NV - 1) z[j] = cs.live(k, j) ? z[j] : 0.f;
+          const float zi = U * R > 1 ? (in ? z[j] : 0.f) : z[j];  // (a wave of one row has none past the end)
+          dw[k][j] = __builtin_fmaf(zi, h[j], dw[k][j]);
+          db[k][j] += zi;
+          z[j] *= w[k][j];
+          c1 += z[j];
+          c2 = __builtin_fmaf(z[j], h[j], c2);
+        }
+      }
+      c1 = row_sum<G>(c1) / n;
+      c2 = row_sum<G>(c2) / n;
+      if (in && a.dx) {
+        T *dr = static_cast<T *>(a.dx) + row * a.lddx;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          float h[V], z[V];
+          if constexpr (TWICE) asm volatile("" : "+v"(xc[u][k]), "+v"(gc[u][k]));  // (or the compiler keeps them)
+          hz(k, h, z);
+#pragma unroll
+          for (int j = 0; j < V; ++j) h[j] = __builtin_fmaf(-h[j], c2, z[j] * w[k][j] - c1) * rs;
+          if (k < NV - 1 || cs.lo < V) stv<T>(dr + cs.c[k], h);
+        }
       }
     }
   }
@@ -442,8 +463,10 @@ bool in_lanes(int64_t D) {
   return D >= vec_of<T>() && D <= 2048;
 }
 
-// f(G, NV as constants) for the row length D: the fewest lanes that hold the row in one vector each,
-// else a whole wave and as many vectors as it takes
+// f(G, NV as constants) for the row length D: the fewest lanes that hold the row in one vector each, else a
+// whole wave and as many vectors as it takes.  (Eight lanes and up to four vectors a lane -- more rows a wave,
+// fewer idle lanes -- was slower wherever rows do not start on cache lines: a store then covers 128 bytes of
+// each of eight rows, partial lines at both ends.  400 K rows of 100 fp32 numbers: 77 us forward against 51.)
 template <typename T, typename F>
 void by_width(int64_t D, F f) {
   constexpr int V = 16 / sizeof(T);
@@ -496,10 +519,16 @@ lpg_status bwd(BwdArgs a, W *dw, W *db, float *part, hipStream_t s) {
   int64_t nblk = 0;
   if (a.M > 0 && in_lanes<T>(a.D)) {
     by_width<T>(a.D, [&](auto g, auto nv) {
-      constexpr int G = decltype(g)::value, NV = decltype(nv)::value, R = 64 / G * kW;
-      auto k = a.relu ? norm_bwd<T, W, G, NV, true> : norm_bwd<T, W, G, NV, false>;
-      const int64_t most = resident_blocks(k, kT);
-      nblk = at_most((a.M + R - 1) / R, most < kPartRows ? most : kPartRows);
+      // Four rows a lane group at a time where a row is one vector a lane, two where it is two: one leaves too
+      // little in flight (400 K x 129 bf16: 82 us with one, 75 with four; 100 K x 1023: 131 with one, 121 with
+      // two) -- unless that would leave CUs without a block (small calls are latency)
+      constexpr int G = decltype(g)::value, NV = decltype(nv)::value, U = NV == 1 ? 4 : (NV == 2 ? 2 : 1);
+      constexpr int R = 64 / G * kW;
+      const bool many = a.M >= (int64_t)R * U * device_cus();
+      auto k = many ? (a.relu ? norm_bwd<T, W, G, NV, true, U> : norm_bwd<T, W, G, NV, false, U>)
+                    : (a.relu ? norm_bwd<T, W, G, NV, true, 1> : norm_bwd<T, W, G, NV, false, 1>);
+      const int64_t rows = many ? R * U : R, most = resident_blocks(k, kT);
+      nblk = at_most((a.M + rows - 1) / rows, most < kPartRows ? most : kPartRows);
       hipLaunchKernelGGL(k, dim3((unsigned)nblk), dim3(kT), 0, s, a);
     });
     LPG_HIP(hipGetLastError());
