@@ -8,17 +8,15 @@
 //
 // The quotient decides borders of whole numbers, so it is decided exactly: x (127 / top) in fp32 is off by
 // less than 127 * 2^-23 < 2^-15.9; where it lies within 2^-15 of a border between two codes (one element
-// in 16000), the vector is done again in fp64, whose correctly rounded 127 x / top is never on the wrong
-// side of a border (two fp32 numbers' quotient is either that border or at least 2^-26 away from it).
+// in 16000), the border's side is found from the exact products instead (at_border).
 //
 // quant_rows: one wave a row, two passes over it (the second from cache).  HBM-bound: x in, q out.
 // fc_i8: MFMA-bound (v_mfma_i32_16x16x64_i8), the k loop of the 16-bit kernel (fc_bf16.hip fc_bf16_p) on
 // bytes: 128-byte k tiles staged by buffer_load ... lds into a swizzled image, two buffers, one barrier a
 // tile in its middle, fragment reads one half tile ahead, transposed fragments (W x A^T: a lane holds four
 // consecutive columns of one row).
-// fc_i8_rows: a few rows (M <= 8) are bound by w's bytes and by latency: every block quantises the rows
-// into LDS itself (no second launch, no q in memory), its first loads of w in flight meanwhile, then a
-// wave a column, 16 bytes of w a lane, v_dot4.
+// fc_i8_row, fc_i8_some: few rows are bound by latency -- the second launch, the k loop's barriers -- and by
+// w's bytes: every block quantises its rows into LDS itself, its first loads of w in flight meanwhile.
 #include "common.h"
 #include "fc_common.h"
 
@@ -47,38 +45,45 @@ struct RowScale {
   }
 };
 
-// n codes of f (inv = 0: zeros, whatever f holds), packed four to a word
-template <int N>
-__device__ __forceinline__ void quant(const float (&f)[N], const RowScale &s, uint32_t (&q)[(N + 3) / 4]) {
-  int c[N];
-  bool near = false;
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const float t = f[j] * s.inv, r = __builtin_rintf(t);
-    near |= fabsf(fabsf(t - r) - 0.5f) < 0x1p-15f;
-    c[j] = (int)r;
-  }
-  if (near) {
-#pragma unroll 1
-    for (int j = 0; j < N; ++j) {
-      const double t = (double)f[j] * 127.0 / (double)s.top;
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i == j) c[i] = (int)__builtin_rint(t);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < (N + 3) / 4; ++j) q[j] = 0;
-#pragma unroll
-  for (int j = 0; j < N; ++j) q[j / 4] |= ((uint32_t)(s.inv == 0.f ? 0 : c[j]) & 0xffu) << (8 * (j & 3));
+// Which side of the border k + 1/2 the quotient 127 |x| / top lies on, exactly: the sign of 254 |x| - (2 k + 1)
+// top, both products with their rounding errors (fma), their difference exact near the border.
+__device__ __forceinline__ int at_border(float x, float top, float t) {
+  const float big = top > 0x1p64f ? 0x1p-32f : 1.f;  // (no product past the range)
+  const float ax = fabsf(x) * big, at = top * big, k = floorf(fabsf(t)), b = 2.f * k + 1.f;
+  const float r = 254.f * ax, p = b * at;
+  const float d = (r - p) + (__builtin_fmaf(254.f, ax, -r) - __builtin_fmaf(b, at, -p));
+  const int n = (int)k;
+  const int q = n + (d > 0.f ? 1 : (d < 0.f ? 0 : (n & 1)));
+  return x < 0.f ? -q : q;
 }
 
-template <typename T>
-__device__ __forceinline__ void ldv(const T *p, float (&f)[16 / sizeof(T)]) {
-  T t[16 / sizeof(T)];
-  __builtin_memcpy(t, p, 16);
+// The codes of f, packed four to a word.  x inv + 1.5 * 2^23 leaves the nearest whole number (halves to even) in
+// the low byte of its bits, two's complement; what it lost tells how near a border was.  (inv = 0: zeros of
+// finite f.)
+template <int N>
+__device__ __forceinline__ void quant(const float (&f)[N], const RowScale &s, uint32_t (&q)[(N + 3) / 4]) {
+  constexpr float kMagic = 12582912.f;
+  uint32_t c[N];
+  float far = 0.f;
 #pragma unroll
-  for (int j = 0; j < (int)(16 / sizeof(T)); ++j) f[j] = (float)t[j];
+  for (int j = 0; j < N; ++j) {
+    const float y = __builtin_fmaf(f[j], s.inv, kMagic);
+    far = fmaxf(far, fabsf(__builtin_fmaf(f[j], s.inv, kMagic - y)));
+    c[j] = __float_as_uint(y);
+  }
+  if (far > 0.5f - 0x1p-15f) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) c[j] = (uint32_t)at_border(f[j], s.top, f[j] * s.inv);
+  }
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j)
+      q[j] = __builtin_amdgcn_perm(c[4 * j + 1], c[4 * j], 0x0c0c0400u) |
+             __builtin_amdgcn_perm(c[4 * j + 3], c[4 * j + 2], 0x04000c0cu);
+  } else {
+    static_assert(N == 1, "vectors of four, or one");
+    q[0] = c[0] & 0xffu;
+  }
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
@@ -89,21 +94,53 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   return v;
 }
 
+// The largest |x| of 16-byte vectors, kept as the types' own bits (their order is that of |x|, NaN on top): two
+// 16-bit elements an operation.
+template <typename T>
+struct Top {
+  typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+  u16x8 m = {0, 0, 0, 0, 0, 0, 0, 0};
+  __device__ __forceinline__ void add(u32x4 v) {
+    if constexpr (sizeof(T) == 2) {
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x8, v & 0x7fff7fffu));
+    } else {
+      m = __builtin_bit_cast(u16x8, __builtin_elementwise_max(__builtin_bit_cast(u32x4, m), v & 0x7fffffffu));
+    }
+  }
+  __device__ __forceinline__ uint32_t bits() const {  // as fp32's
+    uint32_t top = 0;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, abs_bits((float)__builtin_bit_cast(T, (unsigned short)m[j])));
+    } else {
+      const u32x4 w = __builtin_bit_cast(u32x4, m);
+      top = max(max(w[0], w[1]), max(w[2], w[3]));
+    }
+    return top;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack(u32x4 v, float (&f)[16 / sizeof(T)]) {
+  T t[16 / sizeof(T)];
+  __builtin_memcpy(t, &v, 16);
+#pragma unroll
+  for (int j = 0; j < (int)(16 / sizeof(T)); ++j) f[j] = (float)t[j];
+}
+
 // the largest |x| bits of the n elements at p, taken by threads t of nt
 template <typename T>
 __device__ __forceinline__ uint32_t part_max(const T *p, int n, int t, int nt) {
   constexpr int V = 16 / sizeof(T);
-  uint32_t top = 0;
+  Top<T> top;
   const int nv = n / V;
   for (int i = t; i < nv; i += nt) {
-    float f[V];
-    ldv(p + i * V, f);
-#pragma unroll
-    for (int j = 0; j < V; ++j) top = max(top, abs_bits(f[j]));
+    u32x4 v;
+    __builtin_memcpy(&v, p + i * V, 16);
+    top.add(v);
   }
   const int at = nv * V + t;
-  if (at < n) top = max(top, abs_bits((float)p[at]));  // (fewer than V <= nt are left)
-  return top;
+  return max(top.bits(), at < n ? abs_bits((float)p[at]) : 0u);  // (fewer than V <= nt are left)
 }
 
 // ... and their codes, to q (any alignment)
@@ -112,9 +149,11 @@ __device__ __forceinline__ void part_quant(const T *p, int n, int t, int nt, con
   constexpr int V = 16 / sizeof(T);
   const int nv = n / V;
   for (int i = t; i < nv; i += nt) {
+    u32x4 v;
     float f[V];
     uint32_t o[V / 4];
-    ldv(p + i * V, f);
+    __builtin_memcpy(&v, p + i * V, 16);
+    unpack<T>(v, f);
     quant<V>(f, s, o);
     __builtin_memcpy(q + i * V, o, V);
   }
@@ -152,54 +191,62 @@ __global__ __launch_bounds__(256) void quant_rows(QuantArgs a) {
   if (lane == 0) a.scale[row] = s.scale;
 }
 
-// The same for rows of at most 64 NV vectors, held in registers: one pass, all loads of a row in flight.
+// A row of at most 64 NV vectors, held in a wave's registers: all its loads in flight together, read once.
 // Vector i of the row is a vector of x or, from K1 / V on, of x2; the columns that fill no vector are lanes of
 // their own.
 template <typename T, int NV>
+struct HeldRow {
+  static constexpr int V = 16 / sizeof(T);
+  u32x4 v[NV];
+  float rest;
+  __device__ __forceinline__ void load(const T *x, int K1, const T *x2, int K2, int lane) {
+    const int n1 = K1 / V, n2 = K2 / V, r1 = K1 % V, r2 = K2 % V;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = k * 64 + lane;
+      v[k] = u32x4{0u, 0u, 0u, 0u};
+      if (i < n1 + n2) __builtin_memcpy(&v[k], i < n1 ? x + i * V : x2 + (i - n1) * V, 16);
+    }
+    rest = lane < r1 ? (float)x[n1 * V + lane] : (lane < r1 + r2 ? (float)x2[n2 * V + lane - r1] : 0.f);
+  }
+  __device__ __forceinline__ uint32_t top() const {  // of the wave
+    Top<T> t;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) t.add(v[k]);
+    return wave_max(max(t.bits(), abs_bits(rest)));
+  }
+  __device__ __forceinline__ void store(const RowScale &s, int8_t *q, int K1, int K2, int lane) const {
+    const int n1 = K1 / V, n2 = K2 / V, r1 = K1 % V, r2 = K2 % V;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = k * 64 + lane;
+      if (i >= n1 + n2) continue;
+      float f[V];
+      uint32_t o[V / 4];
+      unpack<T>(v[k], f);
+      quant<V>(f, s, o);
+      __builtin_memcpy(q + (i < n1 ? i * V : K1 + (i - n1) * V), o, V);
+    }
+    if (lane < r1 + r2) {
+      const float f[1] = {rest};
+      uint32_t o[1];
+      quant<1>(f, s, o);
+      q[lane < r1 ? n1 * V + lane : K1 + n2 * V + lane - r1] = (int8_t)o[0];
+    }
+  }
+};
+
+template <typename T, int NV>
 __global__ __launch_bounds__(256) void quant_rows_held(QuantArgs a) {
-  constexpr int V = 16 / sizeof(T);
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= a.M) return;
-  const T *x = static_cast<const T *>(a.x) + row * a.ldx;
-  const T *x2 = a.K2 ? static_cast<const T *>(a.x2) + row * a.ldx2 : nullptr;
   int8_t *q = a.q + row * a.ldq;
-  const int n1 = a.K1 / V, n2 = a.K2 / V, r1 = a.K1 % V, r2 = a.K2 % V;
-  u32x4 v[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int i = k * 64 + lane;
-    v[k] = u32x4{0u, 0u, 0u, 0u};
-    if (i < n1 + n2) __builtin_memcpy(&v[k], i < n1 ? x + i * V : x2 + (i - n1) * V, 16);
-  }
-  const float rest[1] = {lane < r1 ? (float)x[n1 * V + lane] : (lane < r1 + r2 ? (float)x2[n2 * V + lane - r1] : 0.f)};
-  uint32_t top = abs_bits(rest[0]);
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    T t[V];
-    __builtin_memcpy(t, &v[k], 16);
-#pragma unroll
-    for (int j = 0; j < V; ++j) top = max(top, abs_bits((float)t[j]));
-  }
-  const RowScale s(wave_max(top));
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int i = k * 64 + lane;
-    if (i >= n1 + n2) continue;
-    T t[V];
-    float f[V];
-    uint32_t o[V / 4];
-    __builtin_memcpy(t, &v[k], 16);
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = (float)t[j];
-    quant<V>(f, s, o);
-    __builtin_memcpy(q + (i < n1 ? i * V : a.K1 + (i - n1) * V), o, V);
-  }
-  if (lane < r1 + r2) {
-    uint32_t o[1];
-    quant<1>(rest, s, o);
-    q[lane < r1 ? n1 * V + lane : a.K1 + n2 * V + lane - r1] = (int8_t)o[0];
-  }
+  HeldRow<T, NV> h;
+  h.load(static_cast<const T *>(a.x) + row * a.ldx, a.K1,
+         a.K2 ? static_cast<const T *>(a.x2) + row * a.ldx2 : nullptr, a.K2, lane);
+  const RowScale s(h.top());
+  h.store(s, q, a.K1, a.K2, lane);
   for (int64_t k = a.K1 + a.K2 + lane; k < a.ldq; k += 64) q[k] = 0;
   if (lane == 0) a.scale[row] = s.scale;
 }
@@ -219,8 +266,8 @@ __device__ __forceinline__ float finish(int acc, float s, float ws, float b, int
   return relu && v < 0.f ? 0.f : v;  // (a NaN stays one)
 }
 
-// WM x WN waves, each FM x FN fragments of 16 x 16.
-template <typename T, int WM, int WN, int FM, int FN>
+// WM x WN waves, each FM x FN fragments of 16 x 16, NB tiles of k in LDS.
+template <typename T, int WM, int WN, int FM, int FN, int NB>
 __global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
   constexpr int NW = WM * WN;
   constexpr int BM = WM * FM * 16, BN = WN * FN * 16;
@@ -229,8 +276,13 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
   static_assert(PA % NW == 0 && PT % NW == 0 && NW % 2 == 0 && PA % 2 == 0, "whole pieces a wave, of one row parity");
   constexpr int EP_PITCH = FN * 16 * 2 + 16;  // 16-bit outputs: the epilogue's image
   constexpr int EP_BYTES = sizeof(T) == 2 ? NW * FM * 16 * EP_PITCH : 0;
-  constexpr int SMEM = 2 * TILE_BYTES > EP_BYTES ? 2 * TILE_BYTES : EP_BYTES;
+  constexpr int SMEM = NB * TILE_BYTES > EP_BYTES ? NB * TILE_BYTES : EP_BYTES;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[SMEM];
+  // The tile's row scales, channel scales and bias, fetched before the k loop: loads after it start the epilogue
+  // with memory latencies.  Not for the 256 tile: the reads back took its k loop to the last register and 12 %
+  // of its rate, its own blocks' length hides the loads.
+  constexpr bool EARLY = BM < 256;
+  __shared__ __attribute__((aligned(16))) float rs[EARLY ? BM : 1], cs[EARLY ? BN : 1], cb[EARLY ? BN : 1];
 
   // XCD-aware order: the blocks of one XCD take a contiguous range of (m, n) tiles
   const int64_t nwg = a.mt * a.nt, bid = blockIdx.x, xcd = bid % 8, q8 = nwg / 8, rr = nwg % 8;
@@ -242,6 +294,14 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int nk = (a.K + BK - 1) / BK, k16 = (a.K + 15) / 16 * 16;
+  if constexpr (EARLY) {
+    for (int i = tid; i < BM; i += 64 * NW) rs[i] = a.scale[m0 + (i < mrows ? i : mrows - 1)];
+    for (int i = tid; i < BN; i += 64 * NW) {
+      const int64_t c = n0 + (i < ncols ? i : ncols - 1);
+      cs[i] = a.wscale[c];
+      cb[i] = a.bias ? a.bias[c] : 0.f;
+    }
+  }
 
   // Descriptors from row m0 of q / row n0 of w, ending with the block's last row: the lane offsets of rows
   // past it are past the range and read zeros.  q's rows hold zeros from K to the tile's end; a row of w
@@ -296,27 +356,30 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
 #pragma unroll
       for (int i = 0; i < FM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bv[j], av[i], acc[i][j], 0, 0, 0);
   };
-  auto barrier = [&]() {  // this wave's DMA landed and its fragment reads returned; then all waves
+  // this wave's DMA landed, but for the latest AHEAD tiles, and its fragment reads returned; then all waves
+  auto barrier = [&](auto ahead) {
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(ahead)::value * PPW) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
 
   i32x4 a0[FM], b0[FN], a1[FM], b1[FN];
-  stage(0, 0);
-  barrier();
-  if (nk > 1) stage(1, 1);
+  static_assert((NB - 1) * PPW < 64, "vmcnt counts to 63");
+#pragma unroll
+  for (int t = 0; t < NB; ++t) stage(t, t);
+  barrier(std::integral_constant<int, NB - 1>());
   rd(0, 0, a0, b0);
   constexpr int NR = FM + FN, NM = FM * FN;
+  int b = 0;
   for (int t = 0; t + 1 < nk; ++t) {
-    const int b = t & 1;
     rd(b, 1, a1, b1);
     mma(a0, b0);
-    barrier();  // tile t + 1 landed everywhere; every wave is done reading buffer b
-    stage(b, t + 2);
-    rd(b ^ 1, 0, a0, b0);
+    barrier(std::integral_constant<int, NB - 2>());  // tile t + 1 landed; every wave is done reading buffer b
+    stage(b, t + NB);
+    b = b + 1 < NB ? b + 1 : 0;
+    rd(b, 0, a0, b0);
     mma(a1, b1);
     if constexpr (NM > PPW + NR) {  // DMA pieces, then the next tile's reads, one a MFMA
 #pragma unroll
@@ -333,7 +396,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  rd((nk - 1) & 1, 1, a1, b1);
+  rd(b, 1, a1, b1);
   mma(a0, b0);
   mma(a1, b1);
   // the image reuses the tile buffers: the last (empty) DMA has landed, every wave is past its reads
@@ -347,16 +410,26 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
   for (int j = 0; j < FN; ++j)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int64_t c = c0 + j * 16 + fq * 4 + r;
-      ws[j][r] = c < a.N ? a.wscale[c] : 0.f;
-      bb[j][r] = a.bias && c < a.N ? a.bias[c] : 0.f;
+      const int l = wn * FN * 16 + j * 16 + fq * 4 + r;
+      if constexpr (EARLY) {
+        ws[j][r] = cs[l];
+        bb[j][r] = cb[l];
+      } else {
+        ws[j][r] = l < ncols ? a.wscale[n0 + l] : 0.f;
+        bb[j][r] = a.bias && l < ncols ? a.bias[n0 + l] : 0.f;
+      }
     }
+  const auto row_scale = [&](int i) {
+    const int l = wm * FM * 16 + i * 16 + fr;
+    if constexpr (EARLY) return rs[l];
+    else return l < mrows ? a.scale[m0 + l] : 0.f;
+  };
   T *y = static_cast<T *>(a.y);
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int64_t row = r0 + i * 16 + fr;
-      const float s = row < a.M ? a.scale[row] : 0.f;
+      const float s = row_scale(i);
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         const int64_t c = c0 + j * 16 + fq * 4;
@@ -378,7 +451,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int64_t row = r0 + i * 16 + fr;
-      const float s = row < a.M ? a.scale[row] : 0.f;
+      const float s = row_scale(i);
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         T v[4];
@@ -415,8 +488,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
 }
 
 struct RowsArgs {
-  int64_t N, ldx, ldx2, ldw, ldy;
-  int M, K1, K2;
+  int64_t M, N, ldx, ldx2, ldw, ldy;
+  int K1, K2;
   const void *x, *x2;
   const int8_t *w;
   const float *wscale, *bias;
@@ -424,75 +497,129 @@ struct RowsArgs {
   int relu;
 };
 
-constexpr int kRows = 8;                // the most rows of fc_i8_rows
-constexpr int kRowsBytes = 48 * 1024;   // ... and the most bytes of their codes in LDS
-
-template <typename T, int RM>
-__global__ __launch_bounds__(256) void fc_i8_rows(RowsArgs a) {
-  extern __shared__ __attribute__((aligned(16))) int8_t qs[];  // RM rows of kp bytes
+// One row: every block quantises it into LDS, then a wave a column.
+constexpr int kRowBytes = 32 * 1024;  // its longest row
+template <typename T>
+__global__ __launch_bounds__(256) void fc_i8_row(RowsArgs a) {
+  extern __shared__ __attribute__((aligned(16))) int8_t qs[];  // kp bytes
   __shared__ uint32_t red[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int K = a.K1 + a.K2, k16 = (K + 15) / 16, kp = (k16 * 16 + 1023) / 1024 * 1024;
+  const int K = a.K1 + a.K2, k16 = (K + 15) / 16, kp = (K + 1023) / 1024 * 1024;
   const int64_t n = (int64_t)blockIdx.x * 4 + wave;
   const i32x4 *w = reinterpret_cast<const i32x4 *>(a.w + (n < a.N ? n : a.N - 1) * a.ldw);
-  // the first chunks of this wave's column, in flight while the rows are quantised
+  // the first chunks of this wave's column, in flight while the row is quantised
   constexpr int P = 4;
   i32x4 pre[P];
 #pragma unroll
   for (int u = 0; u < P; ++u) pre[u] = u * 64 + lane < k16 ? w[u * 64 + lane] : i32x4{0, 0, 0, 0};
-  float scale[RM];
-#pragma unroll
-  for (int m = 0; m < RM; ++m) {
-    if (m < a.M) {
-      const T *x = static_cast<const T *>(a.x) + m * a.ldx;
-      const T *x2 = a.K2 ? static_cast<const T *>(a.x2) + m * a.ldx2 : nullptr;
-      uint32_t top = part_max(x, a.K1, (int)threadIdx.x, 256);
-      if (a.K2) top = max(top, part_max(x2, a.K2, (int)threadIdx.x, 256));
-      top = wave_max(top);
-      __syncthreads();
-      if (lane == 0) red[wave] = top;
-      __syncthreads();
-      const RowScale s(max(max(red[0], red[1]), max(red[2], red[3])));
-      int8_t *q = qs + m * kp;
-      part_quant(x, a.K1, (int)threadIdx.x, 256, s, q);
-      if (a.K2) part_quant(x2, a.K2, (int)threadIdx.x, 256, s, q + a.K1);
-      for (int k = K + (int)threadIdx.x; k < kp; k += 256) q[k] = 0;
-      scale[m] = s.scale;
-    }
-  }
+  const T *x = static_cast<const T *>(a.x), *x2 = static_cast<const T *>(a.x2);
+  uint32_t top = part_max(x, a.K1, (int)threadIdx.x, 256);
+  if (a.K2) top = max(top, part_max(x2, a.K2, (int)threadIdx.x, 256));
+  top = wave_max(top);
+  if (lane == 0) red[wave] = top;
   __syncthreads();
-  int acc[RM];
-#pragma unroll
-  for (int m = 0; m < RM; ++m) acc[m] = 0;
+  const RowScale s(max(max(red[0], red[1]), max(red[2], red[3])));
+  part_quant(x, a.K1, (int)threadIdx.x, 256, s, qs);
+  if (a.K2) part_quant(x2, a.K2, (int)threadIdx.x, 256, s, qs + a.K1);
+  for (int k = K + (int)threadIdx.x; k < kp; k += 256) qs[k] = 0;
+  __syncthreads();
+  int acc = 0;
   const auto dot = [&](i32x4 v, int c) {
+    const i32x4 q = *reinterpret_cast<const i32x4 *>(qs + c * 16);
 #pragma unroll
-    for (int m = 0; m < RM; ++m)
-      if (m < a.M) {
-        const i32x4 q = *reinterpret_cast<const i32x4 *>(qs + m * kp + c * 16);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[m] = __builtin_amdgcn_sdot4(v[r], q[r], acc[m], false);
-      }
+    for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_sdot4(v[r], q[r], acc, false);
   };
 #pragma unroll
   for (int u = 0; u < P; ++u)
     if (u * 64 < k16) dot(pre[u], u * 64 + lane);  // (chunks past k16 are zeros; q is padded to whole kilobytes)
   for (int c = P * 64 + lane; c < k16; c += 64) dot(w[c], c);
 #pragma unroll
-  for (int m = 0; m < RM; ++m) {
-    if (m >= a.M) continue;
-    int v = acc[m];
+  for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o, 64);
+  if (lane == 0 && n < a.N)
+    static_cast<T *>(a.y)[n] = (T)finish(acc, s.scale, a.wscale[n], a.bias ? a.bias[n] : 0.f, a.relu);
+}
+
+// Some rows: a block of eight waves takes 16 rows and 128 columns.  It quantises its rows into LDS, two a wave
+// (every block of the row tile again), then each wave runs 16 columns with w's fragments straight from memory,
+// eight k steps in flight: no barrier and no second launch, which is what a call of this size consists of.
+constexpr int kSomeK = 2048;  // its longest row (16 of them and 16 bytes each in LDS)
+constexpr int kSomeN = 128;
+template <typename T, int NV>
+__global__ __launch_bounds__(512) void fc_i8_some(RowsArgs a) {
+  extern __shared__ __attribute__((aligned(16))) int8_t qs[];  // 16 rows of `pitch` bytes
+  __shared__ float scales[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int P = 8;  // k steps of 64 bytes in flight
+  const int K = a.K1 + a.K2, k16 = (K + 15) / 16 * 16, ks = (K + P * 64 - 1) / (P * 64) * P;
+  const int pitch = ks * 64 + 16;  // (rows 16 bytes apart in the banks)
+  const int64_t m0 = (int64_t)blockIdx.y * 16, n0 = (int64_t)blockIdx.x * kSomeN + wave * 16;
+  const int fr = lane & 15, fq = lane >> 4;
+  HeldRow<T, NV> h[2];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    if (lane == 0 && n < a.N)
-      static_cast<T *>(a.y)[m * a.ldy + n] = (T)finish(v, scale[m], a.wscale[n], a.bias ? a.bias[n] : 0.f, a.relu);
+  for (int i = 0; i < 2; ++i) {
+    const int64_t row = m0 + wave * 2 + i < a.M ? m0 + wave * 2 + i : a.M - 1;
+    h[i].load(static_cast<const T *>(a.x) + row * a.ldx, a.K1,
+              a.K2 ? static_cast<const T *>(a.x2) + row * a.ldx2 : nullptr, a.K2, lane);
+  }
+  const int8_t *w = a.w + (n0 + fr < a.N ? n0 + fr : a.N - 1) * a.ldw;
+  // this lane's four columns: 4 fq .. + 3 of the wave's 16 (the last channel in place of those past N)
+  float ws[4], bb[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int64_t c = n0 + fq * 4 + r < a.N ? n0 + fq * 4 + r : a.N - 1;
+    ws[r] = a.wscale[c];
+    bb[r] = a.bias ? a.bias[c] : 0.f;
+  }
+  const auto load = [&](int t, i32x4(&v)[P]) {
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+      const int k = (t + u) * 64 + fq * 16;
+      v[u] = *reinterpret_cast<const i32x4 *>(w + (k < k16 ? k : 0));  // (past K: anything, q is zero there)
+    }
+  };
+  i32x4 next[P];
+  load(0, next);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const RowScale s(h[i].top());
+    int8_t *q = qs + (wave * 2 + i) * pitch;
+    h[i].store(s, q, a.K1, a.K2, lane);
+    for (int k = K + lane; k < ks * 64; k += 64) q[k] = 0;
+    if (lane == 0) scales[wave * 2 + i] = s.scale;
+  }
+  __syncthreads();
+  i32x4 acc[2] = {i32x4{0, 0, 0, 0}, i32x4{0, 0, 0, 0}};
+  for (int t = 0; t < ks; t += P) {
+    i32x4 v[P], q[P];
+#pragma unroll
+    for (int u = 0; u < P; ++u) v[u] = next[u];
+    if (t + P < ks) load(t + P, next);
+#pragma unroll
+    for (int u = 0; u < P; ++u) q[u] = *reinterpret_cast<const i32x4 *>(qs + fr * pitch + (t + u) * 64 + fq * 16);
+#pragma unroll
+    for (int u = 0; u < P; ++u) acc[u & 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[u], q[u], acc[u & 1], 0, 0, 0);
+  }
+  // a lane holds row fr of the tile and its four columns
+  const int64_t row = m0 + fr, c = n0 + fq * 4;
+  if (row >= a.M) return;
+  T *y = static_cast<T *>(a.y) + row * a.ldy + c;
+  T v[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = (T)finish(acc[0][r] + acc[1][r], scales[fr], ws[r], bb[r], a.relu);
+  if (c + 4 <= a.N) {
+    __builtin_memcpy(y, v, sizeof(v));
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (c + r < a.N) y[r] = v[r];
   }
 }
 
-template <typename T, int WM, int WN, int FM, int FN>
+template <typename T, int WM, int WN, int FM, int FN, int NB>
 void launch_fc(FcArgs a, hipStream_t s) {
   a.mt = (a.M + WM * FM * 16 - 1) / (WM * FM * 16);
   a.nt = (a.N + WN * FN * 16 - 1) / (WN * FN * 16);
-  hipLaunchKernelGGL((fc_i8<T, WM, WN, FM, FN>), dim3((unsigned)(a.mt * a.nt)), dim3(64 * WM * WN), 0, s, a);
+  hipLaunchKernelGGL((fc_i8<T, WM, WN, FM, FN, NB>), dim3((unsigned)(a.mt * a.nt)), dim3(64 * WM * WN), 0, s, a);
 }
 
 int64_t tiles(const FcArgs &a, int64_t b) { return ((a.M + b - 1) / b) * ((a.N + b - 1) / b); }
@@ -500,23 +627,56 @@ int64_t tiles(const FcArgs &a, int64_t b) { return ((a.M + b - 1) / b) * ((a.N +
 template <typename T>
 lpg_status run_fc(const FcArgs &a, hipStream_t s) {
   // the largest tile that still gives most CUs a block
-  if (tiles(a, 256) >= 192) launch_fc<T, 2, 4, 8, 4>(a, s);
-  else if (tiles(a, 128) >= 192) launch_fc<T, 2, 2, 4, 4>(a, s);
-  else launch_fc<T, 2, 2, 2, 2>(a, s);
+  if (tiles(a, 256) >= 192) {
+    // One block a CU: the last round of blocks takes as long as a full one.  Where it would be at most half
+    // full, its rows go to the 128 tile (a quarter of the work, two blocks a CU): 100 K x 1024, K = 2048
+    // 0.370 -> 0.363 ms with the quantisation, 34816 x 1024, K = 1024 85.6 -> 78.9 us; fuller ones lose by it.
+    const int64_t cus = device_cus(), nt = (a.N + 255) / 256, n = tiles(a, 256), mt = n / cus * cus / nt;
+    const int64_t m1 = mt * 256;
+    if (n % cus != 0 && n % cus * 2 <= cus && mt > 0 && m1 < a.M) {
+      FcArgs head = a, tail = a;
+      head.M = m1;
+      tail.M = a.M - m1;
+      tail.q += m1 * a.ldq;
+      tail.scale += m1;
+      tail.y = static_cast<T *>(a.y) + m1 * a.ldy;
+      launch_fc<T, 2, 4, 8, 4, 2>(head, s);
+      LPG_HIP(hipGetLastError());
+      launch_fc<T, 2, 2, 4, 4, 2>(tail, s);
+    } else {
+      launch_fc<T, 2, 4, 8, 4, 2>(a, s);
+    }
+  } else if (tiles(a, 128) >= 192) launch_fc<T, 2, 2, 4, 4, 2>(a, s);
+  else launch_fc<T, 2, 2, 2, 2, 4>(a, s);
   LPG_HIP(hipGetLastError());
   return LPG_OK;
 }
 
 template <typename T>
 lpg_status run_rows(const RowsArgs &a, hipStream_t s) {
-  const int kp = (a.K1 + a.K2 + 1023) / 1024 * 1024;
-  const dim3 g((unsigned)((a.N + 3) / 4)), b(256);
-  if (a.M == 1) hipLaunchKernelGGL((fc_i8_rows<T, 1>), g, b, kp, s, a);
-  else if (a.M == 2) hipLaunchKernelGGL((fc_i8_rows<T, 2>), g, b, 2 * kp, s, a);
-  else if (a.M <= 4) hipLaunchKernelGGL((fc_i8_rows<T, 4>), g, b, a.M * kp, s, a);
-  else hipLaunchKernelGGL((fc_i8_rows<T, kRows>), g, b, a.M * kp, s, a);
+  const int K = a.K1 + a.K2;
+  if (a.M == 1) {
+    hipLaunchKernelGGL(fc_i8_row<T>, dim3((unsigned)((a.N + 3) / 4)), dim3(256), (K + 1023) / 1024 * 1024, s, a);
+  } else {
+    constexpr int V = 16 / sizeof(T);
+    const int nv = (a.K1 / V + a.K2 / V + 63) / 64;
+    const auto go = [&](auto k) {
+      hipLaunchKernelGGL(k, dim3((unsigned)((a.N + kSomeN - 1) / kSomeN), (unsigned)((a.M + 15) / 16)), dim3(512),
+                         16 * ((K + 511) / 512 * 512 + 16), s, a);
+    };
+    if (nv <= 1) go(fc_i8_some<T, 1>);
+    else if (nv <= 2) go(fc_i8_some<T, 2>);
+    else if (nv <= 4) go(fc_i8_some<T, 4>);
+    else go(fc_i8_some<T, 8>);  // (fp32)
+  }
   LPG_HIP(hipGetLastError());
   return LPG_OK;
+}
+
+// What lpg_fc_i8_rows takes: rows that fit its LDS, as many blocks as CUs at most (TODO).
+bool few_rows(int64_t M, int64_t N, int64_t K) {
+  if (M <= 1) return (K + 1023) / 1024 * 1024 <= kRowBytes;
+  return K <= kSomeK && (M + 15) / 16 <= 65535 && (M + 15) / 16 * ((N + kSomeN - 1) / kSomeN) <= device_cus();
 }
 
 constexpr int64_t kMaxK = 131072;  // 131072 * 127^2 < 2^31
@@ -589,20 +749,19 @@ extern "C" lpg_status lpg_fc_i8_rows(int32_t dtype, int64_t M, int64_t N, int64_
                                      int64_t K2, const void *x2, int64_t ldx2, const int8_t *w, int64_t ldw,
                                      const float *wscale, const float *bias, int32_t flags, void *y, int64_t ldy,
                                      void *stream) {
-  LPG_REQUIRE(M >= 0 && M <= kRows && N >= 1 && N <= INT32_MAX && K1 >= 1 && K2 >= 0 && K1 <= kMaxK && K2 <= kMaxK,
-              "lpg_fc_i8_rows: need 0 <= M <= 8, N >= 1, K1 >= 1, K2 >= 0");
+  LPG_REQUIRE(M >= 0 && N >= 1 && N <= INT32_MAX && K1 >= 1 && K2 >= 0 && K1 <= kMaxK && K2 <= kMaxK,
+              "lpg_fc_i8_rows: need M >= 0, 1 <= N < 2^31, K1 >= 1, K2 >= 0, both at most 131072");
   const int64_t K = K1 + K2;
-  if ((K + 1023) / 1024 * 1024 * (M < 1 ? 1 : M) > kRowsBytes) {
-    set_error("lpg_fc_i8_rows: the rows' codes take more than %d bytes (use lpg_quant_i8 and lpg_fc_i8)", kRowsBytes);
-    return LPG_ERR_UNSUPPORTED;
-  }
   LPG_REQUIRE(ldx >= K1 && (K2 == 0 || ldx2 >= K2) && ldy >= N, "lpg_fc_i8_rows: row strides below the columns");
   LPG_REQUIRE(ldw % 16 == 0 && ldw >= (K + 15) / 16 * 16, "lpg_fc_i8_rows: ldw must be a multiple of 16 that holds K");
   LPG_REQUIRE((flags & ~LPG_FC_RELU) == 0, "lpg_fc_i8_rows: unknown flags");
   LPG_REQUIRE(w && wscale && (M == 0 || (x && y && (K2 == 0 || x2))), "lpg_fc_i8_rows: NULL pointer");
   LPG_REQUIRE(aligned16(w), "lpg_fc_i8_rows: w must be 16-byte aligned");
-  const RowsArgs a{N,  ldx, ldx2, ldw,    ldy,  (int)M, (int)K1, (int)K2,
-                   x,  x2,  w,    wscale, bias, y,      (flags & LPG_FC_RELU) ? 1 : 0};
+  if (M > INT32_MAX || !few_rows(M, N, K)) {
+    set_error("lpg_fc_i8_rows: too many or too long rows for one launch (use lpg_quant_i8 and lpg_fc_i8)");
+    return LPG_ERR_UNSUPPORTED;
+  }
+  const RowsArgs a{M, N, ldx, ldx2, ldw, ldy, (int)K1, (int)K2, x, x2, w, wscale, bias, y, (flags & LPG_FC_RELU) ? 1 : 0};
 #define F(T) M == 0 ? LPG_OK : run_rows<T>(a, as_stream(stream))
   LPG_I8_TYPES("lpg_fc_i8_rows", F);
 #undef F

@@ -372,11 +372,11 @@ Tensor linear_i8(const Tensor &x, const Tensor &wq, const Tensor &ws, const OptT
   shape.back() = N;
   Tensor y = at::empty({M, N}, x.options());
   const int32_t type = code_of(x.scalar_type()), flags = relu ? LPG_FC_RELU : 0;
-  if (M > 0 && M <= 8) {
+  if (M > 0) {
     const lpg_status st =
         L.fc_i8_rows(type, M, N, K1, a.data_ptr(), ld(a), K2, ptr(b), K2 ? ld(b) : 0, ptr_of<int8_t>(w),
                      ldw, ptr_of<float>(scale), ptr_of<float>(bb), flags, y.data_ptr(), N, stream_of(x));
-    if (st != LPG_ERR_UNSUPPORTED) {  // (else: rows too long for its LDS)
+    if (st != LPG_ERR_UNSUPPORTED) {  // (else: too many rows for one launch)
       check(st, "lpg_fc_i8_rows");
       return y.view(shape);
     }

@@ -519,10 +519,10 @@ lpg_status bwd(BwdArgs a, W *dw, W *db, float *part, hipStream_t s) {
   int64_t nblk = 0;
   if (a.M > 0 && in_lanes<T>(a.D)) {
     by_width<T>(a.D, [&](auto g, auto nv) {
-      // Four rows a lane group at a time where a row is one vector a lane, two where it is two: one leaves too
-      // little in flight (400 K x 129 bf16: 82 us with one, 75 with four; 100 K x 1023: 131 with one, 121 with
-      // two) -- unless that would leave CUs without a block (small calls are latency)
-      constexpr int G = decltype(g)::value, NV = decltype(nv)::value, U = NV == 1 ? 4 : (NV == 2 ? 2 : 1);
+      // Two rows a lane group at a time where a row is one or two vectors a lane: one leaves too little in flight
+      // (400 K x 129 bf16 82 us with one row, 75 with two; 100 K x 1023 131 and 121) -- unless that would leave
+      // CUs without a block (small calls are latency)
+      constexpr int G = decltype(g)::value, NV = decltype(nv)::value, U = NV <= 2 ? 2 : 1;
       constexpr int R = 64 / G * kW;
       const bool many = a.M >= (int64_t)R * U * device_cus();
       auto k = many ? (a.relu ? norm_bwd<T, W, G, NV, true, U> : norm_bwd<T, W, G, NV, false, U>)

@@ -40,9 +40,11 @@ def test_c_entry_refusals():
     def rw(dtype=2, M=2, N=4, K1=50, x=p, ldx=50, K2=50, x2=p, ldx2=50, w=p, ldw=112, ws=p, flags=0, y=p, ldy=4):
         return L.lpg_fc_i8_rows(dtype, M, N, K1, x, ldx, K2, x2, ldx2, w, ldw, ws, None, flags, y, ldy, None)
 
-    for kw in (dict(dtype=9), dict(M=9), dict(M=-1), dict(N=0), dict(K1=0), dict(K2=-1), dict(ldx=49), dict(ldx2=49),
+    for kw in (dict(dtype=9), dict(M=-1), dict(N=0), dict(K1=0), dict(K2=-1), dict(ldx=49), dict(ldx2=49),
                dict(ldw=96), dict(ldw=104), dict(flags=4), dict(ldy=3), dict(x=None), dict(x2=None), dict(w=None),
                dict(ws=None), dict(y=None), dict(w=p + 4)):
         assert rw(**kw) == 1 and b"lpg_fc_i8_rows" in L.lpg_last_error(), kw
-    assert rw(M=8, K1=6200, ldx=6200, ldw=6256) == 3  # more LDS than the entry takes
+    assert rw(M=2, K1=6200, ldx=6200, ldw=6256) == 3  # more LDS than the entry takes
+    assert rw(M=1, K1=40000, ldx=40000, ldw=40064) == 3
+    assert rw(M=1 << 20) == 3  # too many rows for one launch
     assert rw(M=0, x=None, x2=None, y=None) == 0
