@@ -88,9 +88,26 @@ __device__ __forceinline__ void quant(const float (&f)[N], const RowScale &s, ui
 
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+// the largest over each G lanes, in all of them
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
+}
+template <int G>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  static_assert(G >= 8 && G <= 64, "8 to 64 lanes");
+  v = dpp_max<0xB1>(v);   // quad_perm 1,0,3,2
+  v = dpp_max<0x4E>(v);   // quad_perm 2,3,0,1
+  v = dpp_max<0x141>(v);  // row_half_mirror
+  if constexpr (G > 8) v = dpp_max<0x140>(v);  // row_mirror
+  if constexpr (G > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(r[0], r[1]);
+  }
+  if constexpr (G > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max(r[0], r[1]);
+  }
   return v;
 }
 
@@ -166,6 +183,13 @@ __device__ __forceinline__ void part_quant(const T *p, int n, int t, int nt, con
   }
 }
 
+// zeros from q[k] to q[end], end a multiple of 4, by lanes l of G
+__device__ __forceinline__ void zero_from(int8_t *q, int k, int end, int l, int G) {
+  const int k4 = (k + 3) & ~3;
+  for (int i = k + l; i < k4; i += G) q[i] = 0;
+  for (int i = k4 + l * 4; i < end; i += G * 4) *reinterpret_cast<uint32_t *>(q + i) = 0;
+}
+
 struct QuantArgs {
   int64_t M, ldx, ldx2, ldq;
   int K1, K2;
@@ -184,42 +208,49 @@ __global__ __launch_bounds__(256) void quant_rows(QuantArgs a) {
   int8_t *q = a.q + row * a.ldq;
   uint32_t top = part_max(x, a.K1, lane, 64);
   if (a.K2) top = max(top, part_max(x2, a.K2, lane, 64));
-  const RowScale s(wave_max(top));
+  const RowScale s(lanes_max<64>(top));
   part_quant(x, a.K1, lane, 64, s, q);
   if (a.K2) part_quant(x2, a.K2, lane, 64, s, q + a.K1);
-  for (int64_t k = a.K1 + a.K2 + lane; k < a.ldq; k += 64) q[k] = 0;
+  zero_from(q, a.K1 + a.K2, (int)a.ldq, lane, 64);
   if (lane == 0) a.scale[row] = s.scale;
 }
 
-// A row of at most 64 NV vectors, held in a wave's registers: all its loads in flight together, read once.
-// Vector i of the row is a vector of x or, from K1 / V on, of x2; the columns that fill no vector are lanes of
-// their own.
-template <typename T, int NV>
+// A row of at most G NV vectors, held in the registers of G lanes: all its loads in flight together, read once.
+// Vector i of the row is a vector of x or, from K1 / V on, of x2; the columns that fill no vector (2 V - 2 at
+// most) are single elements of the lanes.
+template <typename T, int G, int NV>
 struct HeldRow {
-  static constexpr int V = 16 / sizeof(T);
+  static constexpr int V = 16 / sizeof(T), NR = (2 * V - 2 + G - 1) / G;
   u32x4 v[NV];
-  float rest;
-  __device__ __forceinline__ void load(const T *x, int K1, const T *x2, int K2, int lane) {
+  float rest[NR];
+  __device__ __forceinline__ void load(const T *x, int K1, const T *x2, int K2, int l) {
     const int n1 = K1 / V, n2 = K2 / V, r1 = K1 % V, r2 = K2 % V;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int i = k * 64 + lane;
+      const int i = k * G + l;
       v[k] = u32x4{0u, 0u, 0u, 0u};
       if (i < n1 + n2) __builtin_memcpy(&v[k], i < n1 ? x + i * V : x2 + (i - n1) * V, 16);
     }
-    rest = lane < r1 ? (float)x[n1 * V + lane] : (lane < r1 + r2 ? (float)x2[n2 * V + lane - r1] : 0.f);
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+      const int i = k * G + l;
+      rest[k] = i < r1 ? (float)x[n1 * V + i] : (i < r1 + r2 ? (float)x2[n2 * V + i - r1] : 0.f);
+    }
   }
-  __device__ __forceinline__ uint32_t top() const {  // of the wave
+  __device__ __forceinline__ uint32_t top() const {  // of the row
     Top<T> t;
 #pragma unroll
     for (int k = 0; k < NV; ++k) t.add(v[k]);
-    return wave_max(max(t.bits(), abs_bits(rest)));
+    uint32_t m = t.bits();
+#pragma unroll
+    for (int k = 0; k < NR; ++k) m = max(m, abs_bits(rest[k]));
+    return lanes_max<G>(m);
   }
-  __device__ __forceinline__ void store(const RowScale &s, int8_t *q, int K1, int K2, int lane) const {
+  __device__ __forceinline__ void store(const RowScale &s, int8_t *q, int K1, int K2, int l) const {
     const int n1 = K1 / V, n2 = K2 / V, r1 = K1 % V, r2 = K2 % V;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int i = k * 64 + lane;
+      const int i = k * G + l;
       if (i >= n1 + n2) continue;
       float f[V];
       uint32_t o[V / 4];
@@ -227,28 +258,32 @@ struct HeldRow {
       quant<V>(f, s, o);
       __builtin_memcpy(q + (i < n1 ? i * V : K1 + (i - n1) * V), o, V);
     }
-    if (lane < r1 + r2) {
-      const float f[1] = {rest};
-      uint32_t o[1];
-      quant<1>(f, s, o);
-      q[lane < r1 ? n1 * V + lane : K1 + n2 * V + lane - r1] = (int8_t)o[0];
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+      const int i = k * G + l;
+      if (i < r1 + r2) {
+        const float f[1] = {rest[k]};
+        uint32_t o[1];
+        quant<1>(f, s, o);
+        q[i < r1 ? n1 * V + i : K1 + n2 * V + i - r1] = (int8_t)o[0];
+      }
     }
   }
 };
 
-template <typename T, int NV>
+template <typename T, int G, int NV>
 __global__ __launch_bounds__(256) void quant_rows_held(QuantArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int l = threadIdx.x % G;
+  const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, at = row < a.M ? row : a.M - 1;
+  HeldRow<T, G, NV> h;
+  h.load(static_cast<const T *>(a.x) + at * a.ldx, a.K1, a.K2 ? static_cast<const T *>(a.x2) + at * a.ldx2 : nullptr,
+         a.K2, l);
+  const RowScale s(h.top());  // (of every lane: rows past the end are the last one again)
   if (row >= a.M) return;
   int8_t *q = a.q + row * a.ldq;
-  HeldRow<T, NV> h;
-  h.load(static_cast<const T *>(a.x) + row * a.ldx, a.K1,
-         a.K2 ? static_cast<const T *>(a.x2) + row * a.ldx2 : nullptr, a.K2, lane);
-  const RowScale s(h.top());
-  h.store(s, q, a.K1, a.K2, lane);
-  for (int64_t k = a.K1 + a.K2 + lane; k < a.ldq; k += 64) q[k] = 0;
-  if (lane == 0) a.scale[row] = s.scale;
+  h.store(s, q, a.K1, a.K2, l);
+  zero_from(q, a.K1 + a.K2, (int)a.ldq, l, G);
+  if (l == 0) a.scale[row] = s.scale;
 }
 
 struct FcArgs {
@@ -515,7 +550,7 @@ __global__ __launch_bounds__(256) void fc_i8_row(RowsArgs a) {
   const T *x = static_cast<const T *>(a.x), *x2 = static_cast<const T *>(a.x2);
   uint32_t top = part_max(x, a.K1, (int)threadIdx.x, 256);
   if (a.K2) top = max(top, part_max(x2, a.K2, (int)threadIdx.x, 256));
-  top = wave_max(top);
+  top = lanes_max<64>(top);
   if (lane == 0) red[wave] = top;
   __syncthreads();
   const RowScale s(max(max(red[0], red[1]), max(red[2], red[3])));
@@ -554,7 +589,7 @@ __global__ __launch_bounds__(512) void fc_i8_some(RowsArgs a) {
   const int pitch = ks * 64 + 16;  // (rows 16 bytes apart in the banks)
   const int64_t m0 = (int64_t)blockIdx.y * 16, n0 = (int64_t)blockIdx.x * kSomeN + wave * 16;
   const int fr = lane & 15, fq = lane >> 4;
-  HeldRow<T, NV> h[2];
+  HeldRow<T, 64, NV> h[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int64_t row = m0 + wave * 2 + i < a.M ? m0 + wave * 2 + i : a.M - 1;
@@ -626,8 +661,11 @@ int64_t tiles(const FcArgs &a, int64_t b) { return ((a.M + b - 1) / b) * ((a.N +
 
 template <typename T>
 lpg_status run_fc(const FcArgs &a, hipStream_t s) {
-  // the largest tile that still gives most CUs a block
-  if (tiles(a, 256) >= 192) {
+  // The largest tile that still gives most CUs a block; but 128 columns where half of the last 256 would be
+  // empty, if that is all there are (100 K x 100, K = 100: 32.5 us against 43.8; x 128, K = 2048 164 and 176) or
+  // the sums are short (60 K x 333, K = 512 58 and 65; K = 2048 145 and 139).
+  const int64_t n128 = (a.N + 127) / 128;
+  if (tiles(a, 256) >= 192 && (n128 % 2 == 0 || (n128 > 1 && a.K > 1024))) {
     // One block a CU: the last round of blocks takes as long as a full one.  Where it would be at most half
     // full, its rows go to the 128 tile (a quarter of the work, two blocks a CU): 100 K x 1024, K = 2048
     // 0.370 -> 0.363 ms with the quantisation, 34816 x 1024, K = 1024 85.6 -> 78.9 us; fuller ones lose by it.
@@ -673,7 +711,9 @@ lpg_status run_rows(const RowsArgs &a, hipStream_t s) {
   return LPG_OK;
 }
 
-// What lpg_fc_i8_rows takes: rows that fit its LDS, as many blocks as CUs at most (TODO).
+// What lpg_fc_i8_rows takes: rows that fit its LDS, as many blocks as CUs at most.  Then it is ahead of the two
+// launches at every size (16 x 128, K = 512 5.2 us against 7.3; 256 x 1024, K = 2048 12.8 and 15.1); with more
+// blocks the rows that each quantises again cost more than the launch (2000 x 512, K = 256 13.6 and 7.3).
 bool few_rows(int64_t M, int64_t N, int64_t K) {
   if (M <= 1) return (K + 1023) / 1024 * 1024 <= kRowBytes;
   return K <= kSomeK && (M + 15) / 16 <= 65535 && (M + 15) / 16 * ((N + kSomeN - 1) / kSomeN) <= device_cus();
@@ -705,23 +745,27 @@ extern "C" lpg_status lpg_quant_i8(int32_t dtype, int64_t M, int64_t K1, const v
   LPG_REQUIRE(aligned16(q), "lpg_quant_i8: q must be 16-byte aligned");
   LPG_REQUIRE((M + 3) / 4 <= INT32_MAX, "lpg_quant_i8: too many rows");
   const QuantArgs a{M, ldx, ldx2, ldq, (int)K1, (int)K2, x, x2, q, scale};
-  const auto go = [&](auto kernel) -> lpg_status {
+  const auto go = [&](auto kernel, int rows) -> lpg_status {
     if (M == 0) return LPG_OK;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((M + 3) / 4)), dim3(256), 0, as_stream(stream), a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((M + rows - 1) / rows)), dim3(256), 0, as_stream(stream), a);
     LPG_HIP(hipGetLastError());
     return LPG_OK;
   };
-  // registers for as many vectors as a lane has, up to 16; longer rows are read twice
+  // the fewest lanes, from 8 on, that hold a row in one vector each, else a wave and up to 16 vectors a lane (100 K
+  // rows of 100 fp16 numbers: 43 us with a wave a row, 15 with 16 lanes); longer rows are read twice
   const auto of = [&](auto t) -> lpg_status {
     using T = decltype(t);
     constexpr int V = 16 / sizeof(T);
-    const int64_t n = (K1 / V + K2 / V + 63) / 64;
-    if (n <= 1) return go(quant_rows_held<T, 1>);
-    if (n <= 2) return go(quant_rows_held<T, 2>);
-    if (n <= 4) return go(quant_rows_held<T, 4>);
-    if (n <= 8) return go(quant_rows_held<T, 8>);
-    if (n <= 16) return go(quant_rows_held<T, 16>);
-    return go(quant_rows<T>);
+    const int64_t n = K1 / V + K2 / V;
+    if (n <= 8) return go(quant_rows_held<T, 8, 1>, 32);
+    if (n <= 16) return go(quant_rows_held<T, 16, 1>, 16);
+    if (n <= 32) return go(quant_rows_held<T, 32, 1>, 8);
+    if (n <= 64) return go(quant_rows_held<T, 64, 1>, 4);
+    if (n <= 128) return go(quant_rows_held<T, 64, 2>, 4);
+    if (n <= 256) return go(quant_rows_held<T, 64, 4>, 4);
+    if (n <= 512) return go(quant_rows_held<T, 64, 8>, 4);
+    if (n <= 1024) return go(quant_rows_held<T, 64, 16>, 4);
+    return go(quant_rows<T>, 4);
   };
 #define F(T) of(T{})
   LPG_I8_TYPES("lpg_quant_i8", F);
