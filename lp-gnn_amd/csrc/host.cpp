@@ -13,8 +13,10 @@
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <stdexcept>
@@ -42,6 +44,7 @@ struct Lib {
   decltype(&lpg_adamw8) adamw8 = nullptr;
   decltype(&lpg_grad_norm_workspace_bytes) grad_norm_workspace_bytes = nullptr;
   decltype(&lpg_grad_norm) grad_norm = nullptr;
+  decltype(&lpg_i8_chunk_rows) i8_chunk_rows = nullptr;
   decltype(&lpg_quant_i8) quant_i8 = nullptr;
   decltype(&lpg_fc_i8) fc_i8 = nullptr;
   decltype(&lpg_fc_i8_rows) fc_i8_rows = nullptr;
@@ -61,6 +64,7 @@ void open(const std::string &path) {
   SYM(adamw8);
   SYM(grad_norm_workspace_bytes);
   SYM(grad_norm);
+  SYM(i8_chunk_rows);
   SYM(quant_i8);
   SYM(fc_i8);
   SYM(fc_i8_rows);
@@ -91,6 +95,12 @@ int64_t ld(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 Tensor rows(const Tensor &t) {
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
   return (r.stride(1) == 1 || r.size(1) == 1) && ld(r) >= r.size(1) ? r : r.contiguous();
+}
+
+bool capturing() {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing(c10::hip::getCurrentHIPStream().stream(), &st) == hipSuccess &&
+         st != hipStreamCaptureStatusNone;
 }
 
 // ------------------------------------------------------------------ layer norm
@@ -167,6 +177,18 @@ Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bia
   REQUIRE(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
           "lpgnn layer_norm: weight and bias must share a type, got ", w.scalar_type(), " and ", b.scalar_type());
   const auto grad = [](const Tensor &t) { return t.defined() && t.requires_grad(); };
+  // A backward that is captured while an eager graph of the same leaves lives would add to their gradients on
+  // the eager graph's stream, out of the capture, which ends the process: refused here, before there is one.
+  if (at::GradMode::is_enabled() && capturing()) {
+    const c10::DeviceGuard guard(x.device());
+    for (const Tensor &t : {x, w, b}) {
+      if (!grad(t) || !t.is_leaf()) continue;
+      const auto acc = torch::autograd::impl::try_get_grad_accumulator(t);
+      const auto stream = acc ? acc->stream() : std::nullopt;
+      REQUIRE(!stream || stream->id() == c10::hip::getCurrentHIPStream(t.get_device()).id(),
+              "lpgnn layer_norm: captured while an eager autograd graph of the same parameters lives; drop it first");
+    }
+  }
   if (at::GradMode::is_enabled() && (grad(x) || grad(w) || grad(b))) return LayerNorm::apply(x, weight, bias, eps, relu);
   return norm_forward(rows(x), w.defined() ? w.contiguous() : w, b.defined() ? b.contiguous() : b, eps, relu, nullptr)
       .view(x.sizes());
@@ -325,19 +347,25 @@ std::pair<Tensor, Tensor> i8_rows(const char *what, const Tensor &x, const OptTe
   return {rows(x), rows(*x2)};
 }
 
-std::pair<Tensor, Tensor> quant(const Tensor &x, const Tensor &x2) {
-  const int64_t M = x.size(0), K1 = x.size(1), K2 = x2.defined() ? x2.size(1) : 0, ldq = (K1 + K2 + 127) / 128 * 128;
-  Tensor q = at::empty({M, ldq}, x.options().dtype(at::kChar)), s = at::empty({M}, x.options().dtype(at::kFloat));
-  check(L.quant_i8(code_of(x.scalar_type()), M, K1, x.data_ptr(), ld(x), K2, ptr(x2), K2 ? ld(x2) : 0,
-                   ptr_of<int8_t>(q), ldq, ptr_of<float>(s), stream_of(x)),
+// rows [at, at + M) of [x | x2] into q [M, ldq] and s [M]
+void quant(const Tensor &x, const Tensor &x2, int64_t at, int64_t M, int8_t *q, int64_t ldq, float *s) {
+  const auto row = [&](const Tensor &t) { return static_cast<char *>(t.data_ptr()) + at * ld(t) * t.element_size(); };
+  const bool two = x2.defined();
+  check(L.quant_i8(code_of(x.scalar_type()), M, x.size(1), row(x), ld(x), two ? x2.size(1) : 0, two ? row(x2) : nullptr,
+                   two ? ld(x2) : 0, q, ldq, s, stream_of(x)),
         "lpg_quant_i8");
-  return {q, s};
+}
+
+int64_t code_pitch(const Tensor &x, const Tensor &x2) {
+  return (x.size(1) + (x2.defined() ? x2.size(1) : 0) + 127) / 128 * 128;
 }
 
 std::pair<Tensor, Tensor> quantize_i8(const Tensor &x, const OptTensor &x2) {
   const auto [a, b] = i8_rows("quantize_i8", x, x2);
   const c10::DeviceGuard guard(x.device());
-  auto [q, s] = quant(a, b);
+  const int64_t M = a.size(0), ldq = code_pitch(a, b);
+  Tensor q = at::empty({M, ldq}, a.options().dtype(at::kChar)), s = at::empty({M}, a.options().dtype(at::kFloat));
+  quant(a, b, 0, M, ptr_of<int8_t>(q), ldq, ptr_of<float>(s));
   return {q.narrow(1, 0, a.size(1) + (b.defined() ? b.size(1) : 0)), s};
 }
 
@@ -382,10 +410,16 @@ Tensor linear_i8(const Tensor &x, const Tensor &wq, const Tensor &ws, const OptT
     }
   }
   if (M > 0) {
-    const auto [q, s] = quant(a, b);
-    check(L.fc_i8(type, M, N, K, ptr_of<int8_t>(q), q.size(1), ptr_of<float>(s), ptr_of<int8_t>(w), ldw,
-                  ptr_of<float>(scale), ptr_of<float>(bb), flags, y.data_ptr(), N, stream_of(x)),
-          "lpg_fc_i8");
+    const int64_t rows = L.i8_chunk_rows(M, N, K), ldq = code_pitch(a, b);
+    Tensor q = at::empty({rows, ldq}, a.options().dtype(at::kChar)), s = at::empty({rows}, a.options().dtype(at::kFloat));
+    for (int64_t at = 0; at < M; at += rows) {
+      const int64_t m = std::min(rows, M - at);
+      quant(a, b, at, m, ptr_of<int8_t>(q), ldq, ptr_of<float>(s));
+      check(L.fc_i8(type, m, N, K, ptr_of<int8_t>(q), ldq, ptr_of<float>(s), ptr_of<int8_t>(w), ldw, ptr_of<float>(scale),
+                    ptr_of<float>(bb), flags, static_cast<char *>(y.data_ptr()) + at * N * y.element_size(), N,
+                    stream_of(x)),
+            "lpg_fc_i8");
+    }
   }
   return y.view(shape);
 }

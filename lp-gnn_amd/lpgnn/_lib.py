@@ -121,6 +121,7 @@ HEADER_SYMBOLS = (
     "lpg_adamw8",
     "lpg_grad_norm_workspace_bytes",
     "lpg_grad_norm",
+    "lpg_i8_chunk_rows",
     "lpg_quant_i8",
     "lpg_fc_i8",
     "lpg_fc_i8_rows",
@@ -369,6 +370,8 @@ def lib() -> ctypes.CDLL:
     L.lpg_grad_norm_workspace_bytes.restype = c_i64
     L.lpg_grad_norm.argtypes = [c_i32, c_i64, c_p, ctypes.c_double, c_p, c_p, c_p, c_p]
     L.lpg_grad_norm.restype = c_i32
+    L.lpg_i8_chunk_rows.argtypes = [c_i64, c_i64, c_i64]
+    L.lpg_i8_chunk_rows.restype = c_i64
     L.lpg_quant_i8.argtypes = [c_i32, c_i64, c_i64, c_p, c_i64, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_p]
     L.lpg_quant_i8.restype = c_i32
     L.lpg_fc_i8.argtypes = [c_i32, c_i64, c_i64, c_i64, c_p, c_i64, c_p, c_p, c_i64, c_p, c_p, c_i32, c_p, c_i64, c_p]

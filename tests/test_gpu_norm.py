@@ -226,3 +226,28 @@ def test_refusals():
     g, = torch.autograd.grad(layer_norm(xr).sum(), xr, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    """A captured forward whose backward would meet the eager graph's gradient accumulators (of another stream) is
+    refused before anything is recorded; after the eager graph is gone it is captured."""
+    from lpgnn import layer_norm
+
+    x = torch.randn(8, 16, device=DEV, requires_grad=True)
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    alive = layer_norm(x, w).sum()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager autograd graph"):
+        with torch.cuda.graph(graph):
+            layer_norm(x, w)
+    torch.cuda.synchronize()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer_norm(x, w)
+        y = layer_norm(y, w)  # the same leaf twice in one capture
+        g, = torch.autograd.grad(y.sum(), w)
+    graph.replay()
+    torch.cuda.synchronize()
+    e = layer_norm(layer_norm(x, w), w)
+    assert torch.equal(y, e) and torch.equal(g, torch.autograd.grad(e.sum(), w)[0])

@@ -194,3 +194,21 @@ def test_refusals():
             linear_i8(*args, **kw)
     with torch.no_grad():
         linear_i8(x.clone().requires_grad_(True), wq, ws)
+
+
+@pytest.mark.parametrize("K1,K2", [(96, 32), (131, 0)])
+def test_more_rows_than_a_chunk(K1, K2):
+    """Rows taken through in several chunks, the last one short: the same bits as chunk by chunk."""
+    from lpgnn import _lib, linear_i8, quantize_i8
+
+    N = 8
+    rows = _lib.lib().lpg_i8_chunk_rows(1 << 40, N, K1 + K2)
+    M = 2 * rows + 777
+    g = torch.Generator(device=DEV).manual_seed(0)
+    wide = torch.randn(M, K1 + K2 + 3, generator=g, device=DEV).half()
+    x, x2 = wide[:, :K1], wide[:, K1 + 1:K1 + 1 + K2] if K2 else None
+    wq, ws = quantize_i8(torch.randn(N, K1 + K2, generator=g, device=DEV))
+    y = linear_i8(x, wq, ws, x2=x2)
+    for a, b in ((0, 100), (rows - 50, rows + 50), (2 * rows - 3, 2 * rows + 60), (M - 30, M)):
+        part = linear_i8(x[a:b], wq, ws, x2=None if x2 is None else x2[a:b])
+        assert torch.equal(y[a:b], part)

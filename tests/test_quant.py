@@ -48,3 +48,14 @@ def test_c_entry_refusals():
     assert rw(M=1, K1=40000, ldx=40000, ldw=40064) == 3
     assert rw(M=1 << 20) == 3  # too many rows for one launch
     assert rw(M=0, x=None, x2=None, y=None) == 0
+
+
+def test_chunk_rows():
+    from lpgnn import _lib
+
+    f = _lib.lib().lpg_i8_chunk_rows
+    assert f(-1, 8, 8) == f(8, 0, 8) == f(8, 8, 0) == -1
+    assert f(0, 8, 8) == 0 and f(100, 1024, 2048) == 100
+    for M, N, K in ((10 ** 5, 1024, 2048), (10 ** 6, 100, 100), (10 ** 6, 2048, 4096), (10 ** 6, 10 ** 6, 131072)):
+        rows = f(M, N, K)
+        assert 0 < rows <= M and (rows == M or rows % 256 == 0)
