@@ -327,7 +327,12 @@ __global__ __launch_bounds__(kT) void sumsq(TableN tab) {
   if (base + kNormChunk <= e.n) {
     float f[U][4];
 #pragma unroll
-    for (int u = 0; u < U; ++u) ld4(g + base + (u * kT + (int)threadIdx.x) * 4, f[u]);
+    for (int u = 0; u < U; ++u) {  // (ordinary loads, the step reads the gradients next: 67 M with the clip 362 -> 325 us)
+      T t[4];
+      __builtin_memcpy(t, g + base + (u * kT + (int)threadIdx.x) * 4, sizeof(t));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[u][j] = (float)t[j];
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) add(f[u]);
   } else {

@@ -321,13 +321,13 @@ std::pair<Tensor, Tensor> clip_scale(const Tensors &gs, double max_norm) {
   std::vector<lpg_tensor> tab(gs.size());
   for (size_t i = 0; i < gs.size(); ++i) tab[i] = {gs[i].data_ptr(), gs[i].numel()};
   const c10::DeviceGuard guard(gs[0].device());
-  Tensor out = at::empty({2}, gs[0].options().dtype(at::kFloat));
-  Tensor ws = at::empty({L.grad_norm_workspace_bytes((int64_t)tab.size(), tab.data()) / 8},
-                        out.options().dtype(at::kDouble));
-  float *o = out.data_ptr<float>();
-  check(L.grad_norm(type, (int64_t)tab.size(), tab.data(), max_norm, o, o + 1, ws.data_ptr(), stream_of(out)),
+  const auto f32 = gs[0].options().dtype(at::kFloat);
+  Tensor norm = at::empty({}, f32), scale = at::empty({}, f32);
+  Tensor ws = at::empty({L.grad_norm_workspace_bytes((int64_t)tab.size(), tab.data()) / 8}, f32.dtype(at::kDouble));
+  check(L.grad_norm(type, (int64_t)tab.size(), tab.data(), max_norm, norm.data_ptr<float>(), scale.data_ptr<float>(),
+                    ws.data_ptr(), stream_of(norm)),
         "lpg_grad_norm");
-  return {out[0], out[1]};
+  return {norm, scale};
 }
 
 // ------------------------------------------------------------------ 8-bit integers
