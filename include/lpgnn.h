@@ -754,7 +754,7 @@ lpg_status lpg_sample_reset(const int64_t *nodes, int64_t ns, int64_t *local, vo
  * Statistics and sums in fp32; NaN and infinity pass through their own row.
  * Backward: dx (NULL = not wanted), dw / db (either may be NULL; M = 0 writes zeros) from x, dy and the
  * forward's mean / rstd; with LPG_NORM_RELU w and b must be the forward's (the mask is recomputed).
- * dw / db need the workspace, deterministic (no atomics). */
+ * dw / db need the workspace, deterministic (no atomics).  No output may overlap an input. */
 #define LPG_BF16 0
 #define LPG_F16 1
 #define LPG_F32 2

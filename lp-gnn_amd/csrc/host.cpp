@@ -18,9 +18,9 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <optional>
 #include <stdexcept>
-#include <unordered_set>
 
 #include "lpgnn.h"
 
@@ -121,17 +121,27 @@ Tensor norm_forward(const Tensor &x, const Tensor &w, const Tensor &b, double ep
   return y;
 }
 
+// What a backward under create_graph hands on: a gradient that depends on what it was computed from by an error
+// (without it a loss that holds a gradient's norm beside other terms would just miss that term's part).
+struct NoSecond : torch::autograd::Function<NoSecond> {
+  static Tensor forward(torch::autograd::AutogradContext *, const Tensor &t, const Tensor &, const Tensor &,
+                        const OptTensor &, const OptTensor &) {
+    return t.view_as(t);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *, torch::autograd::variable_list) {
+    throw std::runtime_error("lpgnn layer_norm: there is no second derivative");
+  }
+};
+
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const OptTensor &weight,
                         const OptTensor &bias, double eps, bool relu) {
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
-    const Tensor xr = rows(x), wc = w.defined() ? w.contiguous() : w, bc = b.defined() ? b.contiguous() : b;
     Tensor stats;
-    Tensor y = norm_forward(xr, wc, bc, eps, relu, &stats);
-    ctx->save_for_backward({xr, wc, bc, stats});
+    Tensor y = norm_forward(x, w, b, eps, relu, &stats);
+    ctx->save_for_backward({x, w, b, stats});
     ctx->saved_data["relu"] = relu;
-    ctx->saved_data["shape"] = x.sizes().vec();
-    return y.view(x.sizes());
+    return y;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
                                                  torch::autograd::variable_list grads) {
@@ -154,7 +164,11 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                            ctx->saved_data["relu"].toBool() ? LPG_NORM_RELU : 0, ptr(dx), D, ptr(dw), ptr(db), ptr(ws),
                            stream_of(x)),
           "lpg_layer_norm_bwd");
-    if (dx.defined()) dx = dx.view(ctx->saved_data["shape"].toIntVector());
+    if (at::GradMode::is_enabled()) {
+      const auto opt = [](const Tensor &t) { return t.defined() ? OptTensor(t) : std::nullopt; };
+      for (Tensor *t : {&dx, &dw, &db})
+        if (t->defined()) *t = NoSecond::apply(*t, x, grads[0], opt(w), opt(b));
+    }
     return {dx, dw, db, Tensor(), Tensor()};
   }
 };
@@ -179,8 +193,8 @@ Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bia
   const auto grad = [](const Tensor &t) { return t.defined() && t.requires_grad(); };
   // A backward that is captured while an eager graph of the same leaves lives would add to their gradients on
   // the eager graph's stream, out of the capture, which ends the process: refused here, before there is one.
+  const c10::DeviceGuard guard(x.device());
   if (at::GradMode::is_enabled() && capturing()) {
-    const c10::DeviceGuard guard(x.device());
     for (const Tensor &t : {x, w, b}) {
       if (!grad(t) || !t.is_leaf()) continue;
       const auto acc = torch::autograd::impl::try_get_grad_accumulator(t);
@@ -189,9 +203,13 @@ Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bia
               "lpgnn layer_norm: captured while an eager autograd graph of the same parameters lives; drop it first");
     }
   }
-  if (at::GradMode::is_enabled() && (grad(x) || grad(w) || grad(b))) return LayerNorm::apply(x, weight, bias, eps, relu);
-  return norm_forward(rows(x), w.defined() ? w.contiguous() : w, b.defined() ? b.contiguous() : b, eps, relu, nullptr)
-      .view(x.sizes());
+  const auto packed = [](const OptTensor &t) { return t ? OptTensor(t->contiguous()) : t; };
+  const Tensor xr = rows(x);
+  const OptTensor wc = packed(weight), bc = packed(bias);
+  const bool graph = at::GradMode::is_enabled() && (grad(x) || grad(w) || grad(b));
+  const Tensor y = graph ? LayerNorm::apply(xr, wc, bc, eps, relu)
+                         : norm_forward(xr, wc.value_or(Tensor()), bc.value_or(Tensor()), eps, relu, nullptr);
+  return x.dim() == 2 ? y : y.view(x.sizes());
 }
 
 // ------------------------------------------------------------------ many tensors
@@ -222,10 +240,37 @@ int32_t params(const char *what, const Tensors &ps) {
   return code_of(type);
 }
 
-void once(const char *what, const Tensors &ps) {
-  std::unordered_set<void *> seen;
-  for (const Tensor &t : ps)
-    REQUIRE(t.numel() == 0 || seen.insert(t.data_ptr()).second, "lpgnn ", what, ": a parameter is in the list twice");
+// No memory that the step writes is another tensor's of the call (two blocks would race for it); read-only
+// tensors may share.
+struct Spans {
+  struct Span {
+    const char *at, *end;
+    bool out;
+  };
+  std::vector<Span> list;
+  void add(const Tensors &ts, bool out) {
+    for (const Tensor &t : ts) {
+      const char *p = static_cast<const char *>(t.data_ptr());
+      if (t.numel() > 0) list.push_back({p, p + t.numel() * t.element_size(), out});
+    }
+  }
+  void check(const char *what) {
+    std::sort(list.begin(), list.end(), [](const Span &a, const Span &b) { return a.at < b.at; });
+    const char *any = nullptr, *out = nullptr;  // the furthest ends so far
+    for (const Span &s : list) {
+      REQUIRE(s.at >= out && !(s.out && s.at < any), "lpgnn ", what,
+              ": tensors of the call overlap (a parameter or a state tensor is in it twice?)");
+      any = std::max(any, s.end);
+      if (s.out) out = std::max(out, s.end);
+    }
+  }
+};
+void apart(const char *what, const Tensors &gs, std::initializer_list<const Tensors *> written) {
+  Spans s;
+  s.list.reserve(gs.size() * (1 + written.size()));
+  s.add(gs, false);
+  for (const Tensors *ts : written) s.add(*ts, true);
+  s.check(what);
 }
 
 lpg_adamw_hyper hyper(const char *what, int64_t step, double lr, std::pair<double, double> betas, double eps,
@@ -258,11 +303,11 @@ void adamw_step(const Tensors &ps, const Tensors &gs, const Tensors &ms, const T
   const lpg_adamw_hyper h = hyper(what, step, lr, betas, eps, weight_decay);
   if (ps.empty()) return;
   const int32_t type = params(what, ps);
-  once(what, ps);
   same(what, "grads", gs, ps, ps[0].scalar_type());
   same(what, "exp_avgs", ms, ps, at::kFloat);
   same(what, "exp_avg_sqs", vs, ps, at::kFloat);
   const float *scale = scale_ptr(what, grad_scale, ps);
+  apart(what, gs, {&ps, &ms, &vs});
   std::vector<lpg_adamw_tensor> tab(ps.size());
   for (size_t i = 0; i < ps.size(); ++i)
     tab[i] = {ps[i].data_ptr(), gs[i].data_ptr(), ptr_of<float>(ms[i]), ptr_of<float>(vs[i]), ps[i].numel()};
@@ -295,7 +340,6 @@ void adamw_step_8bit(const Tensors &ps, const Tensors &gs, const Tensors &m8, co
   const lpg_adamw_hyper h = hyper(what, step, lr, betas, eps, weight_decay);
   if (ps.empty()) return;
   const int32_t type = params(what, ps);
-  once(what, ps);
   REQUIRE(!places || places->size() == ps.size(), "lpgnn ", what, ": ", ps.size(), " params and ", places->size(),
           " places");
   same(what, "grads", gs, ps, ps[0].scalar_type());
@@ -304,6 +348,7 @@ void adamw_step_8bit(const Tensors &ps, const Tensors &gs, const Tensors &m8, co
   same(what, "r8", r8, ps, at::kFloat8_e4m3fn);
   same(what, "r_scales", rs, ps, at::kFloat, true);
   const float *scale = scale_ptr(what, grad_scale, ps);
+  apart(what, gs, {&ps, &m8, &ms, &r8, &rs});
   std::vector<lpg_adamw8_tensor> tab(ps.size());
   for (size_t i = 0; i < ps.size(); ++i)
     tab[i] = {ps[i].data_ptr(),      gs[i].data_ptr(), m8[i].data_ptr(), ptr_of<float>(ms[i]),
@@ -386,12 +431,13 @@ Tensor linear_i8(const Tensor &x, const Tensor &wq, const Tensor &ws, const OptT
   };
   const Tensor scale = vec("ws", ws), bb = bias ? vec("bias", *bias) : Tensor();
   const c10::DeviceGuard guard(x.device());
-  // rows of w on 16-byte borders, each readable to the next one (quantize_i8's are); else a copy that is
+  // rows of w on 16-byte borders, each readable to the next one, within the kernel's pitch (quantize_i8's are);
+  // else a copy that is
   Tensor w = wq;
   const int64_t k16 = (K + 15) / 16 * 16;
   int64_t ldw = N > 1 ? w.stride(0) : k16;
   const bool room = (w.storage_offset() + (N - 1) * ldw + k16) <= (int64_t)w.storage().nbytes();
-  if ((w.stride(1) != 1 && K > 1) || ldw < k16 || ldw % 16 || !room || reinterpret_cast<uintptr_t>(w.data_ptr()) % 16) {
+  if ((w.stride(1) != 1 && K > 1) || ldw < k16 || ldw % 16 || ldw > (1 << 22) || !room || reinterpret_cast<uintptr_t>(w.data_ptr()) % 16) {
     w = at::empty({N, k16}, wq.options()).narrow(1, 0, K);
     w.copy_(wq);
     ldw = k16;

@@ -194,7 +194,8 @@ class GCN_FC(GCNBase):
         """Evaluation in 8-bit integers from here on: the weights of the hidden layers' fully connected parts
         are quantised now (one scale an output channel), their inputs row by row in every forward
         (lpgnn.quant.linear_i8); conv1 (8 + 8 columns), the SpMMs, norms and heads keep their type.  Call it
-        again after the weights change (a forward with other weights raises); ``on=False`` goes back."""
+        again after the weights change (a forward with other weights raises; writes through ``.data`` do not
+        show); ``on=False`` goes back."""
         self._int8 = None
         if on:
             self._int8 = [_conv.quantize_two_direction(c.left2right, c.right2left) for c in self.layers]

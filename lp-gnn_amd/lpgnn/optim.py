@@ -33,8 +33,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 1
                eps: float = 1e-8, weight_decay: float = 1e-2, grad_scale: Tensor | None = None) -> None:
     """One AdamW step (number ``step``, from 1) over lists of contiguous tensors, in place.  params and grads
     float32 or bfloat16 (one type a call), the moments float32; the update is computed in fp32 and rounded
-    once.  ``grad_scale``: a device scalar every gradient is multiplied by (``clip_scale``).  The lists'
-    tensors must not overlap."""
+    once.  ``grad_scale``: a device scalar every gradient is multiplied by (``clip_scale``).  No tensor
+    that is written may overlap another of the call (refused); gradients may share memory."""
     _lib.host().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, grad_scale)
 
 

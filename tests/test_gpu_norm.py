@@ -251,3 +251,39 @@ def test_capture_beside_an_eager_graph_is_refused():
     torch.cuda.synchronize()
     e = layer_norm(layer_norm(x, w), w)
     assert torch.equal(y, e) and torch.equal(g, torch.autograd.grad(e.sum(), w)[0])
+
+
+def test_gradient_of_a_gradient_raises():
+    """Also where it is one term beside others, which have one."""
+    from lpgnn import layer_norm
+
+    x = torch.randn(4, 8, device=DEV, requires_grad=True)
+    w = torch.ones(8, device=DEV, requires_grad=True)
+    y = layer_norm(x, w).square().sum()
+    gx, gw = torch.autograd.grad(y, (x, w), create_graph=True)
+    plain = torch.autograd.grad(layer_norm(x, w).square().sum(), (x, w))
+    assert torch.equal(gx, plain[0]) and torch.equal(gw, plain[1])
+    for g in (gx, gw):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(y + g.square().sum(), x, retain_graph=True)
+
+
+def test_more_elements_than_32_bits_count():
+    """Offsets past 2^31 elements: the last rows are those of a small call."""
+    from lpgnn import layer_norm
+
+    D = 512
+    M = 2**31 // D + 501
+    x = torch.zeros(M, D, dtype=torch.float16, device=DEV)
+    x[-700:].normal_()
+    dy = torch.zeros_like(x)
+    dy[-700:].normal_()
+    w = (torch.rand(D, device=DEV) + 0.5).requires_grad_(True)
+    xs = x[-700:].clone().requires_grad_(True)
+    small = layer_norm(xs, w)
+    gs = torch.autograd.grad(small, xs, dy[-700:])[0]
+    x.requires_grad_(True)
+    y = layer_norm(x, w)
+    g, gw = torch.autograd.grad(y, (x, w), dy)
+    assert torch.equal(y[-700:], small) and torch.equal(g[-700:], gs)
+    assert y[:100].count_nonzero() == 0 and g[:100].count_nonzero() == 0 and gw.isfinite().all()

@@ -398,3 +398,58 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="captured"):
         with torch.cuda.graph(g):
             o.step()
+
+
+def test_overlapping_tensors_are_refused():
+    from lpgnn import optim
+
+    f = torch.zeros(64, device=DEV)
+    t = lambda: torch.zeros(16, device=DEV)
+    ok = dict(params=[f[:16], f[16:32]], grads=[t(), t()], exp_avgs=[t(), t()], exp_avg_sqs=[t(), t()])
+    optim.adamw_step(**ok, step=1)  # (beside each other)
+    g = t()
+    optim.adamw_step(**{**ok, "grads": [g, g]}, step=1)  # (read only)
+    for bad in (dict(params=[f[:16], f[15:31]]), dict(exp_avgs=[g, g]), dict(exp_avg_sqs=ok["exp_avgs"]),
+                dict(grads=[f[4:20], t()]), dict(exp_avgs=[f[40:56], f[32:48]])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            optim.adamw_step(**{**ok, **bad}, step=1)
+    q = [torch.zeros(16, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for _ in range(4)]
+    s = [torch.zeros(1, device=DEV) for _ in range(4)]
+    optim.adamw_step_8bit(ok["params"], ok["grads"], q[:2], s[:2], q[2:], s[2:], step=1)
+    for m8, ms, r8, rs in ((q[:2], s[:2], q[1:3], s[2:]), (q[:2], s[:2], q[2:], s[1:3]), ([q[0], q[0]], s[:2], q[2:], s[2:])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            optim.adamw_step_8bit(ok["params"], ok["grads"], m8, ms, r8, rs, step=1)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_more_elements_than_32_bits_count(bits):
+    """One tensor of more than 2^31 numbers: its last blocks are those of a small call with the same hash inputs
+    (32 bits: of any call), and the norm sees them."""
+    from lpgnn import optim
+
+    n, k = 2**31 + 256 * 5 + 3, 256 * 5 + 3  # (the last k numbers start on a block)
+    p, g = (torch.zeros(n, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    p[-k:].normal_()
+    g[-k:].normal_()
+    p0, g0 = p[-k:].clone(), g[-k:].clone()
+    norm, _ = optim.clip_scale([g], 1.0)
+    want = g0.double().norm()
+    assert abs(norm.double() - want) <= 2.0**-24 * want + 1e-9 * want
+    if bits == 32:
+        st = [torch.zeros(n, device=DEV) for _ in range(2)]
+        s0 = [torch.zeros(k, device=DEV) for _ in range(2)]
+        optim.adamw_step([p], [g], [st[0]], [st[1]], step=1)
+        optim.adamw_step([p0], [g0], [s0[0]], [s0[1]], step=1)
+        assert all(torch.equal(a[-k:], b) for a, b in zip(st, s0))
+    else:
+        f8 = lambda m: torch.zeros(m, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+        sc = lambda m: torch.zeros(-(-m // 256), device=DEV)
+        st, s0 = [f8(n), sc(n), f8(n), sc(n)], [f8(k), sc(k), f8(k), sc(k)]
+        optim.adamw_step_8bit([p], [g], *[[t] for t in st], step=1)
+        optim.adamw_step_8bit([p0], [g0], *[[t] for t in s0], step=1)
+        assert torch.equal(st[1][-6:], s0[1]) and torch.equal(st[3][-6:], s0[3])
+        # the codes' random bits differ by the element: within a step of the format of each other
+        for a, b in ((st[0], s0[0]), (st[2], s0[2])):
+            a, b = a[-k:].float(), b.float()
+            assert ((a - b).abs() <= torch.maximum(a.abs(), b.abs()) / 8 + 2.0**-9).all() and a.count_nonzero() > k // 2
+    assert torch.equal(p[-k:], p0) and p[:1000].count_nonzero() == 0

@@ -212,3 +212,23 @@ def test_more_rows_than_a_chunk(K1, K2):
     for a, b in ((0, 100), (rows - 50, rows + 50), (2 * rows - 3, 2 * rows + 60), (M - 30, M)):
         part = linear_i8(x[a:b], wq, ws, x2=None if x2 is None else x2[a:b])
         assert torch.equal(y[a:b], part)
+
+
+def test_more_elements_than_32_bits_count():
+    """Offsets past 2^31 elements in x and in y, and a weight whose rows are far apart (copied): the bits of small
+    calls."""
+    from lpgnn import linear_i8, quantize_i8
+
+    K = N = 512
+    M = 2**31 // K + 501
+    x = torch.zeros(M, K, dtype=torch.float16, device=DEV)
+    x[-300:].normal_()
+    wq, ws = quantize_i8(torch.randn(N, K, device=DEV))
+    y = linear_i8(x, wq, ws)
+    assert torch.equal(y[-300:], linear_i8(x[-300:].contiguous(), wq, ws)) and y[:1000].count_nonzero() == 0
+    q, s = quantize_i8(x)
+    q0, s0 = quantize_i8(x[-300:].contiguous())
+    assert torch.equal(q[-300:], q0) and torch.equal(s[-300:], s0)
+    far = torch.zeros(3, (1 << 22) + 16, dtype=torch.int8, device=DEV)[:, :K]
+    far.copy_(wq[:3])
+    assert torch.equal(linear_i8(x[-300:], far, ws[:3]), y[-300:, :3])
