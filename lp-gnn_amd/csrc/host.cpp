@@ -13,6 +13,7 @@
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -213,7 +214,24 @@ Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bia
 }
 
 // ------------------------------------------------------------------ many tensors
-using Tensors = std::vector<Tensor>;
+// A Python list or tuple of tensors, borrowed for the call (which keeps the interpreter lock and the list): no
+// reference counts, no vector of copies.
+struct Tensors {
+  pybind11::object fast;
+  PyObject **items = nullptr;
+  size_t n = 0;
+  Tensors(pybind11::handle list, const char *what) {
+    fast = pybind11::reinterpret_steal<pybind11::object>(PySequence_Fast(list.ptr(), "lpgnn: a list of tensors"));
+    if (!fast) throw pybind11::error_already_set();
+    n = (size_t)PySequence_Fast_GET_SIZE(fast.ptr());
+    items = PySequence_Fast_ITEMS(fast.ptr());
+    for (size_t i = 0; i < n; ++i)
+      if (!THPVariable_Check(items[i])) throw pybind11::type_error(c10::str("lpgnn ", what, ": the lists hold tensors"));
+  }
+  size_t size() const { return n; }
+  bool empty() const { return n == 0; }
+  const Tensor &operator[](size_t i) const { return THPVariable_Unpack(items[i]); }
+};
 
 // `ts` beside the parameters `ps`: as many, one type, the parameters' device, contiguous, their sizes (or,
 // scales, one number a block of 256)
@@ -249,7 +267,8 @@ struct Spans {
   };
   std::vector<Span> list;
   void add(const Tensors &ts, bool out) {
-    for (const Tensor &t : ts) {
+    for (size_t i = 0; i < ts.size(); ++i) {
+      const Tensor &t = ts[i];
       const char *p = static_cast<const char *>(t.data_ptr());
       if (t.numel() > 0) list.push_back({p, p + t.numel() * t.element_size(), out});
     }
@@ -293,13 +312,16 @@ const float *scale_ptr(const char *what, const OptTensor &s, const Tensors &ps) 
 
 // the kernels write through pointers: tell autograd (and whatever keeps values by version), as an in-place op
 void written(const Tensors &ts) {
-  for (const Tensor &t : ts)
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  for (size_t i = 0; i < ts.size(); ++i)
+    if (!ts[i].is_inference()) ts[i].unsafeGetTensorImpl()->bump_version();
 }
 
-void adamw_step(const Tensors &ps, const Tensors &gs, const Tensors &ms, const Tensors &vs, int64_t step, double lr,
+using pybind11::handle;
+
+void adamw_step(handle params_, handle grads, handle exp_avgs, handle exp_avg_sqs, int64_t step, double lr,
                 std::pair<double, double> betas, double eps, double weight_decay, const OptTensor &grad_scale) {
   const char *what = "adamw_step";
+  const Tensors ps(params_, what), gs(grads, what), ms(exp_avgs, what), vs(exp_avg_sqs, what);
   const lpg_adamw_hyper h = hyper(what, step, lr, betas, eps, weight_decay);
   if (ps.empty()) return;
   const int32_t type = params(what, ps);
@@ -332,11 +354,11 @@ int64_t rounding_key(int64_t place, int64_t step, uint64_t seed) {
   return mix(step_key(step, seed) + 0x9e3779b9u * (uint32_t)(place + 1));
 }
 
-void adamw_step_8bit(const Tensors &ps, const Tensors &gs, const Tensors &m8, const Tensors &ms, const Tensors &r8,
-                     const Tensors &rs, const std::optional<std::vector<int64_t>> &places, uint64_t seed, int64_t step,
-                     double lr, std::pair<double, double> betas, double eps, double weight_decay,
-                     const OptTensor &grad_scale) {
+void adamw_step_8bit(handle params_, handle grads, handle m8_, handle m_scales, handle r8_, handle r_scales,
+                     const std::optional<std::vector<int64_t>> &places, uint64_t seed, int64_t step, double lr,
+                     std::pair<double, double> betas, double eps, double weight_decay, const OptTensor &grad_scale) {
   const char *what = "adamw_step_8bit";
+  const Tensors ps(params_, what), gs(grads, what), m8(m8_, what), ms(m_scales, what), r8(r8_, what), rs(r_scales, what);
   const lpg_adamw_hyper h = hyper(what, step, lr, betas, eps, weight_decay);
   if (ps.empty()) return;
   const int32_t type = params(what, ps);
@@ -358,8 +380,9 @@ void adamw_step_8bit(const Tensors &ps, const Tensors &gs, const Tensors &m8, co
   written(ps), written(m8), written(ms), written(r8), written(rs);
 }
 
-std::pair<Tensor, Tensor> clip_scale(const Tensors &gs, double max_norm) {
+std::pair<Tensor, Tensor> clip_scale(handle grads, double max_norm) {
   const char *what = "clip_scale";
+  const Tensors gs(grads, what);
   REQUIRE(!gs.empty(), "lpgnn clip_scale: no gradients");
   REQUIRE(max_norm >= 0, "lpgnn clip_scale: max_norm must not be negative, got ", max_norm);
   const int32_t type = params(what, gs);
