@@ -20,6 +20,9 @@
 // infinity gets the scale NaN: the state stays visibly bad, as it does in 32 bits.  The parameter update
 // uses the moments before they are rounded.
 //
+// 67 M numbers: 277 us with fp32 moments (6.8 TB/s), 166-186 with 8-bit ones (5.8), the norm 46 (5.8); 4.2 M: 8-bit
+// step 17, norm 8 + 4; 70 K in 22 tensors 4.2 us.
+//
 // The norm is summed in 64 bits: products of fp32 numbers are exact there, and the sum's order does not
 // show in the 32-bit result, so the clip factor is the same however the tensors are split.
 #include "common.h"

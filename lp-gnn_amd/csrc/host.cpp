@@ -1,10 +1,11 @@
 // lpgnn._host: the host side of calls that are bound by it.
 //
 // A layer norm of a small graph or the optimizer step of a small model is a few microseconds of GPU time;
-// checking the arguments, the autograd node and the launch from Python took 20 us a layer norm, 80 more
-// for its backward (a Python node in the engine's thread waits for the interpreter lock) and 40 us a step
-// over 24 tensors.  Here the same checks, the autograd node and the call of the C entry (include/lpgnn.h,
-// resolved from the library that lpgnn._lib loads) run in C++: 8, 45 and 9 us.
+// checking the arguments, the autograd node and the launch from Python took 14 us a layer norm, 142 its
+// training pass (a Python node in the engine's thread waits for the interpreter lock) and 42 a step over 24
+// tensors.  Here the same checks, the autograd node and the call of the C entry (include/lpgnn.h, resolved
+// from the library that lpgnn._lib loads) run in C++: 5, 30 to 65 (the engine's hand-over between threads;
+// 14 of it are this file's and the launches) and 6 us.
 //
 // Every refusal is a RuntimeError before any device work; device, stream and allocator are torch's current
 // ones of the tensors' device.
