@@ -819,8 +819,8 @@ lpg_status lpg_grad_norm(int32_t dtype, int64_t count, const lpg_tensor *tensors
  * lpg_fc_i8: y = act((sum_k q[m,k] w[n,k]) scale[m] wscale[n] + bias[n]), the sum exact in 32-bit
  * integers, y of `dtype` [M, N]; w int8 [N, ldw], ldw a multiple of 16, 16-byte aligned, each row readable
  * to K rounded up to 16 (what lies past K meets zeros of q); K <= 131072; bias NULL = 0; flags: LPG_FC_RELU.
- * lpg_i8_chunk_rows: the rows to take through the two at a time (at most M): q of a chunk stays in cache
- * between them, and a chunk fills whole rounds of the GPU's CUs.
+ * lpg_i8_chunk_rows: how many of M rows to take through the two next: q of a chunk stays in cache between
+ * them, and a chunk fills whole rounds of the GPU's CUs (the last one is up to a quarter longer).
  * lpg_fc_i8_rows: both in one launch, without q, for rows few and short enough that this is faster; else
  * LPG_ERR_UNSUPPORTED (use the other two). */
 int64_t lpg_i8_chunk_rows(int64_t M, int64_t N, int64_t K);

@@ -15,8 +15,9 @@
 // fc_i8: MFMA- and LDS-bound (v_mfma_i32_16x16x64_i8), the k loop of the 16-bit kernel (fc_bf16.hip fc_bf16_p) on
 // bytes: 128-byte k tiles staged by buffer_load ... lds into a swizzled image, two buffers (four in the small tile),
 // one barrier a tile in its middle, fragment reads one half tile ahead, transposed fragments (W x A^T: a lane holds
-// four consecutive columns of one row).  16384 x 2048, K = 4096: 107 us, 2.56 POPS; 32768 x 1024, K = 2048: 69 us,
-// 2.0 (1.2 us a k tile and 15 us a round of blocks for its first loads and its stores).
+// four consecutive columns of one row), stores straight from registers.  16384 x 2048, K = 4096: 108 us, 2.55 POPS;
+// 100 K x 1024, K = 2048: 194 us, 2.16 (a k tile takes 1.4 us, of which the MFMAs 0.85 at 2.4 GHz; the first round's
+// loads and the last one's stores are not hidden).
 // fc_i8_row, fc_i8_some: few rows are bound by latency -- the second launch, the k loop's barriers -- and by
 // w's bytes: every block quantises its rows into LDS itself, its first loads of w in flight meanwhile.  One row of
 // 2048 to 1024 columns: 3.8 us.
@@ -299,53 +300,53 @@ struct FcArgs {
   int relu;
 };
 
+// 64 floats from p on (those past its n bytes: zeros) to LDS
+__device__ __forceinline__ void dma4(uint64_t p, uint32_t n, float *lds, uint32_t voff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef __attribute__((address_space(3))) void lds_v;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      reinterpret_cast<void *>(((uint64_t)hi << 32) | lo), (short)0, (int)__builtin_amdgcn_readfirstlane(n), 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_v *)lds, 4, voff, 0, 0, 0);
+#endif
+}
+
 __device__ __forceinline__ float finish(int acc, float s, float ws, float b, int relu) {
   const float v = ((float)acc * s) * ws + b;
   return relu && v < 0.f ? 0.f : v;  // (a NaN stays one)
 }
 
-// WM x WN waves, each FM x FN fragments of 16 x 16, NB tiles of k in LDS.
-template <typename T, int WM, int WN, int FM, int FN, int NB>
-__global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
+// WM x WN waves, each FM x FN fragments of 16 x 16, NB tiles of k in LDS.  ON: a block takes output tiles blockIdx.x,
+// + gridDim.x, ... in one stream of k tiles, those of the next output tile in flight while this one is stored; else
+// blockIdx.x is the only one.
+template <typename T, int WM, int WN, int FM, int FN, int NB, bool ON>
+__global__ __launch_bounds__(64 * WM * WN, 2) void fc_i8(FcArgs a) {
   constexpr int NW = WM * WN;
   constexpr int BM = WM * FM * 16, BN = WN * FN * 16;
   constexpr int A_BYTES = BM * BK, TILE_BYTES = A_BYTES + BN * BK;
   constexpr int PA = BM / 8, PT = PA + BN / 8, PPW = PT / NW;  // 1-KiB pieces: A, all, a wave
   static_assert(PA % NW == 0 && PT % NW == 0 && NW % 2 == 0 && PA % 2 == 0, "whole pieces a wave, of one row parity");
-  constexpr int EP_PITCH = FN * 16 * 2 + 16;  // 16-bit outputs: the epilogue's image
-  constexpr int EP_BYTES = sizeof(T) == 2 ? NW * FM * 16 * EP_PITCH : 0;
-  constexpr int SMEM = NB * TILE_BYTES > EP_BYTES ? NB * TILE_BYTES : EP_BYTES;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[SMEM];
-  // The tile's row scales, channel scales and bias, fetched before the k loop: loads after it start the epilogue
-  // with memory latencies.  Not for the 256 tile: the reads back took its k loop to the last register and 12 %
-  // of its rate, its own blocks' length hides the loads.
-  constexpr bool EARLY = BM < 256;
-  __shared__ __attribute__((aligned(16))) float rs[EARLY ? BM : 1], cs[EARLY ? BN : 1], cb[EARLY ? BN : 1];
-
-  // XCD-aware order: the blocks of one XCD take a contiguous range of (m, n) tiles
-  const int64_t nwg = a.mt * a.nt, bid = blockIdx.x, xcd = bid % 8, q8 = nwg / 8, rr = nwg % 8;
-  const int64_t wgid = (xcd < rr ? xcd * (q8 + 1) : rr * (q8 + 1) + (xcd - rr) * q8) + bid / 8;
-  const int64_t m0 = wgid / a.nt * BM, n0 = wgid % a.nt * BN;
-  const int64_t mrows = a.M - m0 < BM ? a.M - m0 : BM, ncols = a.N - n0 < BN ? a.N - n0 : BN;
+  // Behind the k tiles: the output tiles' row scales, channel scales and biases, staged with their first k tile
+  // (NB output tiles ahead of the one that is stored, where a tile has one k tile).  One array for all: beside a
+  // second one the compiler tells apart what the DMA writes, and waits for it before every read.
+  constexpr int SC = BM + 2 * BN, NS = NB + 1;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[NB * TILE_BYTES + NS * SC * 4];
+  float *const sc = reinterpret_cast<float *>(smem + NB * TILE_BYTES);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int nk = (a.K + BK - 1) / BK, k16 = (a.K + 15) / 16 * 16;
-  if constexpr (EARLY) {
-    for (int i = tid; i < BM; i += 64 * NW) rs[i] = a.scale[m0 + (i < mrows ? i : mrows - 1)];
-    for (int i = tid; i < BN; i += 64 * NW) {
-      const int64_t c = n0 + (i < ncols ? i : ncols - 1);
-      cs[i] = a.wscale[c];
-      cb[i] = a.bias ? a.bias[c] : 0.f;
-    }
-  }
+  const uint32_t nwg = (uint32_t)(a.mt * a.nt), nt = (uint32_t)a.nt;
 
-  // Descriptors from row m0 of q / row n0 of w, ending with the block's last row: the lane offsets of rows
-  // past it are past the range and read zeros.  q's rows hold zeros from K to the tile's end; a row of w
-  // may end before the tile does (the lanes of those chunks get an offset past the range).
-  const uint64_t pa = (uint64_t)(a.q + m0 * a.ldq), pw = (uint64_t)(a.w + n0 * a.ldw);
-  const uint32_t na = (uint32_t)((mrows - 1) * a.ldq + nk * BK), nw = (uint32_t)((ncols - 1) * a.ldw + k16);
+  // XCD-aware order: the blocks of one XCD take a contiguous range of (m, n) tiles
+  const auto origin = [&](uint32_t tile, int64_t &m0, int64_t &n0) {
+    const uint32_t xcd = tile % 8, q8 = nwg / 8, rr = nwg % 8;
+    const uint32_t at = (xcd < rr ? xcd * (q8 + 1) : rr * (q8 + 1) + (xcd - rr) * q8) + tile / 8;
+    m0 = (int64_t)(at / nt) * BM;
+    n0 = (int64_t)(at % nt) * BN;
+  };
+
   uint32_t vo[PPW];
 #pragma unroll
   for (int p = 0; p < PPW; ++p) {
@@ -354,26 +355,48 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
     vo[p] = (uint32_t)(row * (q < PA ? a.ldq : a.ldw) + swz(row, lane & 7) * 16);
   }
   const int chunk_at = swz((wave & 1) * 8 + (lane >> 3), lane & 7) * 16;  // of all this wave's pieces
-  auto stage = [&](int b, int t) {
-    const bool ok = t < nk;  // past the last tile: the same instructions with an empty range
-    t = ok ? t : nk - 1;
+
+  // The next k tile to stage: of output tile s_tile, its number s_k.  Descriptors from row m0 of q / row n0 of w,
+  // ending with the tile's last row: the lane offsets of rows past it are past the range and read zeros.  q's rows
+  // hold zeros from K to the k tile's end; a row of w may end before it does (the lanes of those chunks get an
+  // offset past the range).  Past the last one: the same instructions with empty ranges.
+  uint32_t s_tile = blockIdx.x, s_scales = 0;
+  int s_k = 0;
+  uint64_t pa = 0, pw = 0;
+  uint32_t na = 0, nw = 0;
+  const auto open_tile = [&]() {  // of s_tile, for its first k tile
+      const bool some = s_tile < nwg;
+      int64_t m0, n0;
+      origin(some ? s_tile : 0, m0, n0);
+      const int64_t mrows = a.M - m0 < BM ? a.M - m0 : BM, ncols = a.N - n0 < BN ? a.N - n0 : BN;
+      pa = (uint64_t)(a.q + m0 * a.ldq);
+      pw = (uint64_t)(a.w + n0 * a.ldw);
+      na = some ? (uint32_t)((mrows - 1) * a.ldq + nk * BK) : 0u;
+      nw = some ? (uint32_t)((ncols - 1) * a.ldw + k16) : 0u;
+      for (int i = wave; i < SC / 64; i += NW) {
+        const bool row = i < BM / 64, col = !row && i < (BM + BN) / 64;
+        const float *p = row ? a.scale + m0 : (col ? a.wscale + n0 : a.bias + (a.bias ? n0 : 0));
+        const int at = (row ? i : (col ? i - BM / 64 : i - (BM + BN) / 64)) * 64;
+        const uint32_t n = some && (row || col || a.bias) ? (uint32_t)(row ? mrows : ncols) * 4 : 0u;
+        dma4((uint64_t)p, n, sc + s_scales * SC + i * 64, (uint32_t)(at + lane) * 4);
+      }
+      s_scales = s_scales + 1 < NS ? s_scales + 1 : 0;
+      s_k = 0;
+      s_tile = some ? s_tile + gridDim.x : nwg;
+  };
+  const auto stage = [&](int b) {
     unsigned char *base = smem + b * TILE_BYTES;
-    const uint32_t ra = ok ? na : 0u, rw = ok ? nw : 0u;
-    const bool in = chunk_at < k16 - t * BK;
+    const bool in = chunk_at < k16 - s_k * BK;
 #pragma unroll
     for (int p = 0; p < PPW; ++p) {
       const int q = wave + NW * p;
-      if (p < PA / NW) dma16(pa, ra, base + q * 1024, vo[p], t * BK);
-      else dma16(pw, rw, base + q * 1024, in ? vo[p] : 0x7fffff00u, t * BK);
+      if (p < PA / NW) dma16(pa, ON || s_k < nk ? na : 0u, base + q * 1024, vo[p], s_k * BK);
+      else dma16(pw, ON || s_k < nk ? nw : 0u, base + q * 1024, in ? vo[p] : 0x7fffff00u, s_k * BK);
     }
+    ++s_k;
   };
 
   i32x4 acc[FM][FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-
   const int fr = lane & 15, fq = lane >> 4;
   auto rd = [&](int b, int s, i32x4(&av)[FM], i32x4(&bv)[FN]) {  // half s (64 k) of buffer b
     const unsigned char *As = smem + b * TILE_BYTES, *Bs = As + A_BYTES;
@@ -394,28 +417,44 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
 #pragma unroll
       for (int i = 0; i < FM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bv[j], av[i], acc[i][j], 0, 0, 0);
   };
-  // this wave's DMA landed, but for the latest AHEAD tiles, and its fragment reads returned; then all waves
-  auto barrier = [&](auto ahead) {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(ahead)::value * PPW) : "memory");
+  // this wave's DMA landed, but for the latest `later` operations, and its fragment reads returned; then all waves
+  auto arrive = [&](auto later) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(later)::value) : "memory");
+  };
+  auto meet = [&]() {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
 
+  T *y = static_cast<T *>(a.y);
   i32x4 a0[FM], b0[FN], a1[FM], b1[FN];
   static_assert((NB - 1) * PPW < 64, "vmcnt counts to 63");
 #pragma unroll
-  for (int t = 0; t < NB; ++t) stage(t, t);
-  barrier(std::integral_constant<int, NB - 1>());
+  for (int t = 0; t < NB; ++t) {
+    if (t == 0 || (ON && s_k == nk)) open_tile();
+    stage(t);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  arrive(std::integral_constant<int, (NB - 1) * PPW>());
+  meet();
   rd(0, 0, a0, b0);
   constexpr int NR = FM + FN, NM = FM * FN;
-  int b = 0;
-  for (int t = 0; t + 1 < nk; ++t) {
+  // stores of a whole tile, which the first wait after them leaves out (its k tile was staged before them)
+  constexpr int STORES = FM * FN / (sizeof(T) == 2 ? 2 : 1), AFTER = (NB - 2) * PPW + STORES;
+  static_assert(AFTER < 64, "vmcnt counts to 63");
+  int b = 0, scales = 0;
+  bool stored = false;  // a whole tile was, since the last wait
+  const auto step = [&]() {  // one k tile
+    __builtin_amdgcn_sched_barrier(0);
     rd(b, 1, a1, b1);
     mma(a0, b0);
-    barrier(std::integral_constant<int, NB - 2>());  // tile t + 1 landed; every wave is done reading buffer b
-    stage(b, t + NB);
+    __builtin_amdgcn_sched_barrier(0);
+    if (ON && stored) arrive(std::integral_constant<int, AFTER>());
+    else arrive(std::integral_constant<int, (NB - 2) * PPW>());
+    stored = false;
+    meet();  // the next k tile landed; every wave is done reading buffer b
+    stage(b);
     b = b + 1 < NB ? b + 1 : 0;
     rd(b, 0, a0, b0);
     mma(a1, b1);
@@ -433,96 +472,108 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void fc_i8(FcArgs a) {
       __builtin_amdgcn_sched_group_barrier(0x008, NM - PPW - NR, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
-  }
-  rd(b, 1, a1, b1);
-  mma(a0, b0);
-  mma(a1, b1);
-  // the image reuses the tile buffers: the last (empty) DMA has landed, every wave is past its reads
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-
-  // a lane holds row 16 i + fr, columns 16 j + 4 fq .. + 3 of its wave's part
-  const int64_t r0 = m0 + wm * FM * 16, c0 = n0 + wn * FN * 16;
-  float ws[FN][4], bb[FN][4];
-#pragma unroll
-  for (int j = 0; j < FN; ++j)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int l = wn * FN * 16 + j * 16 + fq * 4 + r;
-      if constexpr (EARLY) {
-        ws[j][r] = cs[l];
-        bb[j][r] = cb[l];
-      } else {
-        ws[j][r] = l < ncols ? a.wscale[n0 + l] : 0.f;
-        bb[j][r] = a.bias && l < ncols ? a.bias[n0 + l] : 0.f;
-      }
-    }
-  const auto row_scale = [&](int i) {
-    const int l = wm * FM * 16 + i * 16 + fr;
-    if constexpr (EARLY) return rs[l];
-    else return l < mrows ? a.scale[m0 + l] : 0.f;
   };
-  T *y = static_cast<T *>(a.y);
-  if constexpr (sizeof(T) == 4) {
+  for (uint32_t tile = blockIdx.x; tile < nwg; tile += gridDim.x) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int64_t row = r0 + i * 16 + fr;
-      const float s = row_scale(i);
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const int64_t c = c0 + j * 16 + fq * 4;
-        float v[4];
+      for (int j = 0; j < FN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    if constexpr (ON) {
+#pragma unroll 1
+      for (int t = 0; t < nk; ++t) {
+        if (s_k == nk) open_tile();
+        step();
+      }
+    } else {
+      for (int t = 0; t + 1 < nk; ++t) step();
+      rd(b, 1, a1, b1);
+      mma(a0, b0);
+      mma(a1, b1);
+    }
+
+    // a lane holds row 16 i + er, columns 16 j + 4 eq .. + 3 of its wave's part (its place found anew: nothing of the
+    // epilogue is kept in registers through the k loop)
+    int el = lane;
+    asm volatile("" : "+v"(el));
+    const int er = el & 15, eq = el >> 4;
+    int64_t m0, n0;
+    origin(tile, m0, n0);
+    stored = m0 + BM <= a.M && n0 + BN <= a.N;
+    const int64_t r0 = m0 + wm * FM * 16, c0 = n0 + wn * FN * 16;
+    const float *rs = sc + scales * SC + wm * FM * 16 + er, *cs = sc + scales * SC + BM + wn * FN * 16 + eq * 4, *cb = cs + BN;
+    scales = scales + 1 < NS ? scales + 1 : 0;
+    float ws[FN][4], bb[FN][4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = finish(acc[i][j][r], s, ws[j][r], bb[j][r], a.relu);
-        if (row < a.M && c + 4 <= a.N) {
-          __builtin_memcpy(y + row * a.ldy + c, v, 16);
-        } else if (row < a.M) {
+    for (int j = 0; j < FN; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (c + r < a.N) y[row * a.ldy + c + r] = v[r];
+      for (int r = 0; r < 4; ++r) ws[j][r] = cs[j * 16 + r], bb[j][r] = cb[j * 16 + r];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int64_t row = r0 + i * 16 + er;
+        const float s = rs[i * 16];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const int64_t c = c0 + j * 16 + eq * 4;
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = finish(acc[i][j][r], s, ws[j][r], bb[j][r], a.relu);
+          if (row < a.M && c + 4 <= a.N) {
+            __builtin_memcpy(y + row * a.ldy + c, v, 16);
+          } else if (row < a.M) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (c + r < a.N) y[row * a.ldy + c + r] = v[r];
+          }
+        }
+      }
+    } else {
+      // Lanes eq = 0 .. 3 hold columns 4 eq .. + 3 of fragments j and j + 1; two exchanges between them leave columns
+      // 8 eq .. + 7 of the 32 in each: rows leave as 16-byte stores, 64 bytes a row
+      static_assert(FN % 2 == 0, "fragments in pairs");
+      // (not past the caches where a row's 64 bytes are parts of two lines)
+      const bool lines = (a.ldy & 63) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 127) == 0;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int64_t row = r0 + i * 16 + er;
+        const float s = rs[i * 16];
+#pragma unroll
+        for (int j = 0; j < FN; j += 2) {
+          uint32_t o[2][2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            T v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = (T)finish(acc[i][j + h][r], s, ws[j + h][r], bb[j + h][r], a.relu);
+            __builtin_memcpy(o[h], v, 8);
+          }
+          u32x4 out;
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            const auto x = __builtin_amdgcn_permlane32_swap(o[0][d], o[1][d], false, false);
+            const auto z = __builtin_amdgcn_permlane16_swap(x[0], x[1], false, false);
+            out[d] = z[0];
+            out[2 + d] = z[1];
+          }
+          const int64_t c = c0 + j * 16 + eq * 8;
+          if (row >= a.M || c >= a.N) continue;
+          T *p = y + row * a.ldy + c;
+          if (c + 8 <= a.N) {
+            if (lines) __builtin_nontemporal_store(out, reinterpret_cast<u32x4 *>(p));
+            else __builtin_memcpy(p, &out, 16);
+          } else {
+            T e[8];
+            __builtin_memcpy(e, &out, 16);
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+              if (c + r < a.N) p[r] = e[r];
+          }
         }
       }
     }
-  } else {
-    // through LDS, so that rows leave as 16-byte stores
-    unsigned char *img = smem + wave * (FM * 16 * EP_PITCH);
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int64_t row = r0 + i * 16 + fr;
-      const float s = row_scale(i);
-#pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        T v[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = (T)finish(acc[i][j][r], s, ws[j][r], bb[j][r], a.relu);
-        uint2 o;
-        __builtin_memcpy(&o, v, 8);
-        *reinterpret_cast<uint2 *>(img + (i * 16 + fr) * EP_PITCH + (j * 16 + fq * 4) * 2) = o;
-      }
-    }
-    __builtin_amdgcn_wave_barrier();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    constexpr int CPR = FN * 16 / 8;  // 16-byte chunks a row
-    const bool al = (a.ldy & 7) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
-#pragma unroll
-    for (int it = 0; it < FM * 16 * CPR / 64; ++it) {
-      const int k = it * 64 + lane, lr = k / CPR, ch = k % CPR;
-      const int64_t row = r0 + lr, c = c0 + ch * 8;
-      const u32x4 v = *reinterpret_cast<const u32x4 *>(img + lr * EP_PITCH + ch * 16);
-      if (row >= a.M || c >= a.N) continue;
-      T *p = y + row * a.ldy + c;
-      if (c + 8 <= a.N) {
-        if (al) __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(p));
-        else __builtin_memcpy(p, &v, 16);
-      } else {
-        T e[8];
-        __builtin_memcpy(e, &v, 16);
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (c + r < a.N) p[r] = e[r];
-      }
-    }
+    if constexpr (!ON) break;
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the empty DMAs have landed before the LDS is another block's)
 }
 
 struct RowsArgs {
@@ -657,7 +708,17 @@ template <typename T, int WM, int WN, int FM, int FN, int NB>
 void launch_fc(FcArgs a, hipStream_t s) {
   a.mt = (a.M + WM * FM * 16 - 1) / (WM * FM * 16);
   a.nt = (a.N + WN * FN * 16 - 1) / (WN * FN * 16);
-  hipLaunchKernelGGL((fc_i8<T, WM, WN, FM, FN, NB>), dim3((unsigned)(a.mt * a.nt)), dim3(64 * WM * WN), 0, s, a);
+  const int64_t n = a.mt * a.nt;
+  // The 256 tile leaves a CU room for one block: where there is more than a round of them, as many blocks as CUs that
+  // go on (100 K x 1024, K = 2048 212 -> 193 us; one round 36.5 without, 37.9 with it).  Of the smaller tiles other
+  // blocks of the CU fill the time of the stores.
+  if constexpr (WM * FM * 16 == 256) {
+    if (n > device_cus()) {
+      hipLaunchKernelGGL((fc_i8<T, WM, WN, FM, FN, NB, true>), dim3((unsigned)device_cus()), dim3(64 * WM * WN), 0, s, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((fc_i8<T, WM, WN, FM, FN, NB, false>), dim3((unsigned)n), dim3(64 * WM * WN), 0, s, a);
 }
 
 int64_t tiles(const FcArgs &a, int64_t b) { return ((a.M + b - 1) / b) * ((a.N + b - 1) / b); }
@@ -670,8 +731,8 @@ lpg_status run_fc(const FcArgs &a, hipStream_t s) {
   const int64_t n128 = (a.N + 127) / 128;
   if (tiles(a, 256) >= 192 && (n128 % 2 == 0 || (n128 > 1 && a.K > 1024))) {
     // One block a CU: the last round of blocks takes as long as a full one.  Where it would be at most half
-    // full, its rows go to the 128 tile (a quarter of the work, two blocks a CU): 100 K x 1024, K = 2048
-    // 0.370 -> 0.363 ms with the quantisation, 34816 x 1024, K = 1024 85.6 -> 78.9 us; fuller ones lose by it.
+    // full, its rows go to the 128 tile (a quarter of the work, two blocks a CU): 34816 x 1024, K = 1024 (an eighth of
+    // a round left) 54 -> 49 us, 24576 x 1024, K = 2048 (half) 56 -> 50; 26624 rows (five eighths) 57 -> 61.
     const int64_t cus = device_cus(), nt = (a.N + 255) / 256, n = tiles(a, 256), mt = n / cus * cus / nt;
     const int64_t m1 = mt * 256;
     if (n % cus != 0 && n % cus * 2 <= cus && mt > 0 && m1 < a.M) {
@@ -738,16 +799,17 @@ using namespace lpg;
     return LPG_ERR_INVALID;                                                              \
   } while (0)
 
-// 64 MiB of codes: written by the one kernel and read by the other they stay in the 256 MiB of last-level cache
-// beside w and the streams of x and y.  Whole rounds of 256-row tiles.  100 K x 1024, K = 2048 0.341 -> 0.316 ms,
-// 200 K x 2048, K = 4096 1.91 -> 1.84, against all rows at once; half of it costs launches, twice gains half.
+// 96 MiB of codes: written by the one kernel and read by the other they stay in the 256 MiB of last-level cache
+// beside w and the streams of x and y.  Whole rounds of 256-row tiles, and up to a quarter more in place of a short
+// last chunk.  200 K x 2048, K = 4096 with 48 / 64 / 96 / 128 MiB 2.03 / 1.86 / 1.83 / 1.92 ms, 200 K x 1024, K = 2048
+// 0.64 / 0.61 / 0.59 / 0.67; half a chunk more instead of a quarter: 130 K x 1024, K = 1024 0.257 against 0.220.
 extern "C" int64_t lpg_i8_chunk_rows(int64_t M, int64_t N, int64_t K) {
   if (M < 0 || N < 1 || K < 1) return -1;
   const int64_t ldq = (K + 127) / 128 * 128, nt = (N + 255) / 256, cus = device_cus();
-  const int64_t round = (cus + nt - 1) / nt * 256;  // rows of one round
-  int64_t rows = (((int64_t)64 << 20) / ldq) / round * round;
-  rows = rows < round ? round : rows;
-  return M < rows + rows / 2 ? M : rows;  // (no short second chunk)
+  const int64_t rounds = ((int64_t)96 << 20) / ldq / 256 * nt / cus;
+  int64_t rows = (rounds < 1 ? 1 : rounds) * cus / nt * 256;
+  rows = rows < 256 ? 256 : rows;
+  return M < rows + rows / 4 ? M : rows;
 }
 
 extern "C" lpg_status lpg_quant_i8(int32_t dtype, int64_t M, int64_t K1, const void *x, int64_t ldx, int64_t K2,

@@ -480,10 +480,10 @@ Tensor linear_i8(const Tensor &x, const Tensor &wq, const Tensor &ws, const OptT
     }
   }
   if (M > 0) {
-    const int64_t rows = L.i8_chunk_rows(M, N, K), ldq = code_pitch(a, b);
-    Tensor q = at::empty({rows, ldq}, a.options().dtype(at::kChar)), s = at::empty({rows}, a.options().dtype(at::kFloat));
-    for (int64_t at = 0; at < M; at += rows) {
-      const int64_t m = std::min(rows, M - at);
+    const int64_t rows = L.i8_chunk_rows(M, N, K), most = rows < M ? rows + rows / 4 : M, ldq = code_pitch(a, b);
+    Tensor q = at::empty({most, ldq}, a.options().dtype(at::kChar)), s = at::empty({most}, a.options().dtype(at::kFloat));
+    for (int64_t at = 0, m; at < M; at += m) {
+      m = std::min(L.i8_chunk_rows(M - at, N, K), most);
       quant(a, b, at, m, ptr_of<int8_t>(q), ldq, ptr_of<float>(s));
       check(L.fc_i8(type, m, N, K, ptr_of<int8_t>(q), ldq, ptr_of<float>(s), ptr_of<int8_t>(w), ldw, ptr_of<float>(scale),
                     ptr_of<float>(bb), flags, static_cast<char *>(y.data_ptr()) + at * N * y.element_size(), N,
