@@ -297,7 +297,8 @@ struct FcArgs {
   const float *scale, *wscale, *bias;
   void *y;
   int64_t mt, nt;
-  int relu;
+  float lo;
+  int past;  // y is stored past the caches
 };
 
 // 64 floats from p on (those past its n bytes: zeros) to LDS
@@ -311,9 +312,15 @@ __device__ __forceinline__ void dma4(uint64_t p, uint32_t n, float *lds, uint32_
 #endif
 }
 
-__device__ __forceinline__ float finish(int acc, float s, float ws, float b, int relu) {
-  const float v = ((float)acc * s) * ws + b;
-  return relu && v < 0.f ? 0.f : v;  // (a NaN stays one)
+// lo: 0 with the ReLU, -infinity without (a NaN stays one)
+__device__ __forceinline__ float finish(int acc, float s, float ws, float b, float lo) {
+  return __builtin_elementwise_maximum(((float)acc * s) * ws + b, lo);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pair(float a, float b) {  // as two 16-bit numbers
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef T t16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), t16x2));
 }
 
 // WM x WN waves, each FM x FN fragments of 16 x 16, NB tiles of k in LDS.  ON: a block takes output tiles blockIdx.x,
@@ -507,70 +514,64 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fc_i8(FcArgs a) {
     for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) ws[j][r] = cs[j * 16 + r], bb[j][r] = cb[j * 16 + r];
-    if constexpr (sizeof(T) == 4) {
+    // all stores of the wave's part: of a whole tile past the caches or through them, or whatever exists of it
+    const auto store = [&](auto how) {
+      constexpr bool WHOLE = decltype(how)::value < 2, PAST = decltype(how)::value == 0;  // (PAST: of 16 bits)
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         const int64_t row = r0 + i * 16 + er;
         const float s = rs[i * 16];
+        const auto v = [&](int j, int r) { return finish(acc[i][j][r], s, ws[j][r], bb[j][r], a.lo); };
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          const int64_t c = c0 + j * 16 + eq * 4;
-          float v[4];
+          for (int j = 0; j < FN; ++j) {
+            const int64_t c = c0 + j * 16 + eq * 4;
+            const float out[4] = {v(j, 0), v(j, 1), v(j, 2), v(j, 3)};
+            T *p = y + row * a.ldy + c;
+            if (WHOLE || (row < a.M && c + 4 <= a.N)) {
+              __builtin_memcpy(p, out, 16);
+            } else if (row < a.M && c < a.N) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = finish(acc[i][j][r], s, ws[j][r], bb[j][r], a.relu);
-          if (row < a.M && c + 4 <= a.N) {
-            __builtin_memcpy(y + row * a.ldy + c, v, 16);
-          } else if (row < a.M) {
+              for (int r = 0; r < 4; ++r)
+                if (c + r < a.N) p[r] = out[r];
+            }
+          }
+        } else {
+          // Lanes eq = 0 .. 3 hold columns 4 eq .. + 3 of fragments j and j + 1; two exchanges between them leave
+          // columns 8 eq .. + 7 of the 32 in each: rows leave as 16-byte stores, 64 bytes a row
+          static_assert(FN % 2 == 0, "fragments in pairs");
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (c + r < a.N) y[row * a.ldy + c + r] = v[r];
+          for (int j = 0; j < FN; j += 2) {
+            u32x4 out;
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+              const auto x = __builtin_amdgcn_permlane32_swap(pair<T>(v(j, 2 * d), v(j, 2 * d + 1)),
+                                                              pair<T>(v(j + 1, 2 * d), v(j + 1, 2 * d + 1)), false, false);
+              const auto z = __builtin_amdgcn_permlane16_swap(x[0], x[1], false, false);
+              out[d] = z[0];
+              out[2 + d] = z[1];
+            }
+            const int64_t c = c0 + j * 16 + eq * 8;
+            __builtin_amdgcn_sched_barrier(0);  // (a store as soon as its numbers are: 16384 x 1024, K = 128 14.8 -> 12.9 us)
+            T *p = y + row * a.ldy + c;
+            if constexpr (PAST) {
+              __builtin_nontemporal_store(out, reinterpret_cast<u32x4 *>(p));
+            } else if (WHOLE || (row < a.M && c + 8 <= a.N)) {
+              __builtin_memcpy(p, &out, 16);
+            } else if (row < a.M && c < a.N) {
+              T e[8];
+              __builtin_memcpy(e, &out, 16);
+#pragma unroll
+              for (int r = 0; r < 8; ++r)
+                if (c + r < a.N) p[r] = e[r];
+            }
           }
         }
       }
-    } else {
-      // Lanes eq = 0 .. 3 hold columns 4 eq .. + 3 of fragments j and j + 1; two exchanges between them leave columns
-      // 8 eq .. + 7 of the 32 in each: rows leave as 16-byte stores, 64 bytes a row
-      static_assert(FN % 2 == 0, "fragments in pairs");
-      // (not past the caches where a row's 64 bytes are parts of two lines)
-      const bool lines = (a.ldy & 63) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 127) == 0;
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int64_t row = r0 + i * 16 + er;
-        const float s = rs[i * 16];
-#pragma unroll
-        for (int j = 0; j < FN; j += 2) {
-          uint32_t o[2][2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            T v[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (T)finish(acc[i][j + h][r], s, ws[j + h][r], bb[j + h][r], a.relu);
-            __builtin_memcpy(o[h], v, 8);
-          }
-          u32x4 out;
-#pragma unroll
-          for (int d = 0; d < 2; ++d) {
-            const auto x = __builtin_amdgcn_permlane32_swap(o[0][d], o[1][d], false, false);
-            const auto z = __builtin_amdgcn_permlane16_swap(x[0], x[1], false, false);
-            out[d] = z[0];
-            out[2 + d] = z[1];
-          }
-          const int64_t c = c0 + j * 16 + eq * 8;
-          if (row >= a.M || c >= a.N) continue;
-          T *p = y + row * a.ldy + c;
-          if (c + 8 <= a.N) {
-            if (lines) __builtin_nontemporal_store(out, reinterpret_cast<u32x4 *>(p));
-            else __builtin_memcpy(p, &out, 16);
-          } else {
-            T e[8];
-            __builtin_memcpy(e, &out, 16);
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-              if (c + r < a.N) p[r] = e[r];
-          }
-        }
-      }
-    }
+    };
+    if (sizeof(T) == 2 && stored && a.past) store(std::integral_constant<int, 0>());
+    else if (stored) store(std::integral_constant<int, 1>());
+    else store(std::integral_constant<int, 2>());
     if constexpr (!ON) break;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the empty DMAs have landed before the LDS is another block's)
@@ -583,7 +584,7 @@ struct RowsArgs {
   const int8_t *w;
   const float *wscale, *bias;
   void *y;
-  int relu;
+  float lo;
 };
 
 // One row: every block quantises it into LDS, then a wave a column.
@@ -625,7 +626,7 @@ __global__ __launch_bounds__(256) void fc_i8_row(RowsArgs a) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o, 64);
   if (lane == 0 && n < a.N)
-    static_cast<T *>(a.y)[n] = (T)finish(acc, s.scale, a.wscale[n], a.bias ? a.bias[n] : 0.f, a.relu);
+    static_cast<T *>(a.y)[n] = (T)finish(acc, s.scale, a.wscale[n], a.bias ? a.bias[n] : 0.f, a.lo);
 }
 
 // Some rows: a block of eight waves takes 16 rows and 128 columns.  It quantises its rows into LDS, two a wave
@@ -694,7 +695,7 @@ __global__ __launch_bounds__(512) void fc_i8_some(RowsArgs a) {
   T *y = static_cast<T *>(a.y) + row * a.ldy + c;
   T v[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) v[r] = (T)finish(acc[0][r] + acc[1][r], scales[fr], ws[r], bb[r], a.relu);
+  for (int r = 0; r < 4; ++r) v[r] = (T)finish(acc[0][r] + acc[1][r], scales[fr], ws[r], bb[r], a.lo);
   if (c + 4 <= a.N) {
     __builtin_memcpy(y, v, sizeof(v));
   } else {
@@ -860,7 +861,14 @@ extern "C" lpg_status lpg_fc_i8(int32_t dtype, int64_t M, int64_t N, int64_t K, 
   LPG_REQUIRE(w && wscale && (M == 0 || (q && scale && y)), "lpg_fc_i8: NULL pointer");
   LPG_REQUIRE(aligned16(q) && aligned16(w), "lpg_fc_i8: q and w must be 16-byte aligned");
   LPG_REQUIRE(((M + 63) / 64) <= INT32_MAX / ((N + 63) / 64), "lpg_fc_i8: too many tiles");
-  const FcArgs a{M, N, ldq, ldw, ldy, (int)K, q, w, scale, wscale, bias, y, 0, 0, (flags & LPG_FC_RELU) ? 1 : 0};
+  // Past the caches go outputs that would push out the codes: not short sums' (100 K x 1024, K = 64 60 us through
+  // them, 73 past them), not small ones (20000 x 1024, K = 1024 41 and 43; 200 K x 2048, K = 1024 629 and 537), only
+  // rows on whole lines (30000 x 1000, K = 2000 62 us through them, 86 past them), not fp32's (their stores take
+  // longer than the codes: 100 K x 512, K = 256 83 and 99).
+  const int past = dtype != LPG_F32 && K > 128 && M * N > (int64_t)32 << 20 && ldy % 64 == 0 &&
+                   reinterpret_cast<uintptr_t>(y) % 128 == 0;
+  const FcArgs a{M, N, ldq, ldw, ldy, (int)K, q, w, scale, wscale, bias, y, 0, 0,
+                 (flags & LPG_FC_RELU) ? 0.f : -INFINITY, past};
 #define F(T) M == 0 ? LPG_OK : run_fc<T>(a, as_stream(stream))
   LPG_I8_TYPES("lpg_fc_i8", F);
 #undef F
@@ -882,7 +890,7 @@ extern "C" lpg_status lpg_fc_i8_rows(int32_t dtype, int64_t M, int64_t N, int64_
     set_error("lpg_fc_i8_rows: too many or too long rows for one launch (use lpg_quant_i8 and lpg_fc_i8)");
     return LPG_ERR_UNSUPPORTED;
   }
-  const RowsArgs a{M, N, ldx, ldx2, ldw, ldy, (int)K1, (int)K2, x, x2, w, wscale, bias, y, (flags & LPG_FC_RELU) ? 1 : 0};
+  const RowsArgs a{M, N, ldx, ldx2, ldw, ldy, (int)K1, (int)K2, x, x2, w, wscale, bias, y, (flags & LPG_FC_RELU) ? 0.f : -INFINITY};
 #define F(T) M == 0 ? LPG_OK : run_rows<T>(a, as_stream(stream))
   LPG_I8_TYPES("lpg_fc_i8_rows", F);
 #undef F
