@@ -333,10 +333,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fc_i8(FcArgs a) {
   constexpr int A_BYTES = BM * BK, TILE_BYTES = A_BYTES + BN * BK;
   constexpr int PA = BM / 8, PT = PA + BN / 8, PPW = PT / NW;  // 1-KiB pieces: A, all, a wave
   static_assert(PA % NW == 0 && PT % NW == 0 && NW % 2 == 0 && PA % 2 == 0, "whole pieces a wave, of one row parity");
-  // Behind the k tiles: the output tiles' row scales, channel scales and biases, staged with their first k tile
-  // (NB output tiles ahead of the one that is stored, where a tile has one k tile).  One array for all: beside a
-  // second one the compiler tells apart what the DMA writes, and waits for it before every read.
-  constexpr int SC = BM + 2 * BN, NS = NB + 1;
+  // Behind the k tiles: the output tiles' row scales, channel scales and biases, staged with their first k tile.  Where a
+  // tile has one k tile that is NB tiles ahead, before the barrier that all waves' stores of the tile before are behind:
+  // NB + 2 tiles' are alive.  One array for all: beside a second one the compiler tells apart what the DMA writes, and
+  // waits for it before every read.
+  constexpr int SC = BM + 2 * BN, NS = ON ? NB + 2 : 1;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[NB * TILE_BYTES + NS * SC * 4];
   float *const sc = reinterpret_cast<float *>(smem + NB * TILE_BYTES);
 
@@ -372,24 +373,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fc_i8(FcArgs a) {
   uint64_t pa = 0, pw = 0;
   uint32_t na = 0, nw = 0;
   const auto open_tile = [&]() {  // of s_tile, for its first k tile
-      const bool some = s_tile < nwg;
-      int64_t m0, n0;
-      origin(some ? s_tile : 0, m0, n0);
-      const int64_t mrows = a.M - m0 < BM ? a.M - m0 : BM, ncols = a.N - n0 < BN ? a.N - n0 : BN;
-      pa = (uint64_t)(a.q + m0 * a.ldq);
-      pw = (uint64_t)(a.w + n0 * a.ldw);
-      na = some ? (uint32_t)((mrows - 1) * a.ldq + nk * BK) : 0u;
-      nw = some ? (uint32_t)((ncols - 1) * a.ldw + k16) : 0u;
-      for (int i = wave; i < SC / 64; i += NW) {
-        const bool row = i < BM / 64, col = !row && i < (BM + BN) / 64;
-        const float *p = row ? a.scale + m0 : (col ? a.wscale + n0 : a.bias + (a.bias ? n0 : 0));
-        const int at = (row ? i : (col ? i - BM / 64 : i - (BM + BN) / 64)) * 64;
-        const uint32_t n = some && (row || col || a.bias) ? (uint32_t)(row ? mrows : ncols) * 4 : 0u;
-        dma4((uint64_t)p, n, sc + s_scales * SC + i * 64, (uint32_t)(at + lane) * 4);
-      }
-      s_scales = s_scales + 1 < NS ? s_scales + 1 : 0;
-      s_k = 0;
-      s_tile = some ? s_tile + gridDim.x : nwg;
+    const bool some = s_tile < nwg;
+    int64_t m0, n0;
+    origin(some ? s_tile : 0, m0, n0);
+    const int64_t mrows = a.M - m0 < BM ? a.M - m0 : BM, ncols = a.N - n0 < BN ? a.N - n0 : BN;
+    pa = (uint64_t)(a.q + m0 * a.ldq);
+    pw = (uint64_t)(a.w + n0 * a.ldw);
+    na = some ? (uint32_t)((mrows - 1) * a.ldq + nk * BK) : 0u;
+    nw = some ? (uint32_t)((ncols - 1) * a.ldw + k16) : 0u;
+    for (int i = wave; i < SC / 64; i += NW) {
+      const bool row = i < BM / 64, col = !row && i < (BM + BN) / 64;
+      const float *p = row ? a.scale + m0 : (col ? a.wscale + n0 : a.bias + (a.bias ? n0 : 0));
+      const int at = (row ? i : (col ? i - BM / 64 : i - (BM + BN) / 64)) * 64;
+      const uint32_t n = some && (row || col || a.bias) ? (uint32_t)(row ? mrows : ncols) * 4 : 0u;
+      dma4((uint64_t)p, n, sc + s_scales * SC + i * 64, (uint32_t)(at + lane) * 4);
+    }
+    s_scales = s_scales + 1 < NS ? s_scales + 1 : 0;
+    s_k = 0;
+    s_tile = some ? s_tile + gridDim.x : nwg;
   };
   const auto stage = [&](int b) {
     unsigned char *base = smem + b * TILE_BYTES;
@@ -711,11 +712,14 @@ void launch_fc(FcArgs a, hipStream_t s) {
   a.nt = (a.N + WN * FN * 16 - 1) / (WN * FN * 16);
   const int64_t n = a.mt * a.nt;
   // The 256 tile leaves a CU room for one block: where there is more than a round of them, as many blocks as CUs that
-  // go on (100 K x 1024, K = 2048 212 -> 193 us; one round 36.5 without, 37.9 with it).  Of the smaller tiles other
-  // blocks of the CU fill the time of the stores.
-  if constexpr (WM * FM * 16 == 256) {
-    if (n > device_cus()) {
-      hipLaunchKernelGGL((fc_i8<T, WM, WN, FM, FN, NB, true>), dim3((unsigned)device_cus()), dim3(64 * WM * WN), 0, s, a);
+  // go on (100 K x 1024, K = 2048 212 -> 193 us; one round 36.5 without, 37.9 with it).  Two blocks of the 128 tile
+  // fill each other's time of the stores, but for short sums in many rounds (147 K x 1600, K = 38 174 -> 146; 60 K x
+  // 384, K = 128, 2.7 rounds, 14.6 without, 15.4 with it).
+  constexpr int BM = WM * FM * 16;
+  if constexpr (BM >= 128) {
+    const int64_t blocks = (BM == 256 ? 1 : 2) * device_cus();
+    if (n > blocks * (BM == 256 ? 1 : 4)) {
+      hipLaunchKernelGGL((fc_i8<T, WM, WN, FM, FN, NB, true>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, s, a);
       return;
     }
   }

@@ -232,3 +232,28 @@ def test_more_elements_than_32_bits_count():
     far = torch.zeros(3, (1 << 22) + 16, dtype=torch.int8, device=DEV)[:, :K]
     far.copy_(wq[:3])
     assert torch.equal(linear_i8(x[-300:], far, ws[:3]), y[-300:, :3])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("M,N,K", [(256 * 150 + 5, 512, 100), (256 * 150, 512, 129), (256 * 280, 512, 260),
+                                   (300 * 128 + 1, 1100, 40), (256 * 131, 1024, 384)])
+def test_blocks_that_go_on_to_further_tiles(M, N, K, dtype):
+    """More tiles than blocks, of one k tile and of several, whole ones and cut ones, outputs on lines and off: the
+    codes' product by the C entry is that of few rows at a time."""
+    from lpgnn import _lib, linear_i8, quantize_i8
+
+    g = torch.Generator(device=DEV).manual_seed(M + N + K)
+    x = (torch.randn(M, K, generator=g, device=DEV) * torch.rand(M, 1, generator=g, device=DEV)).to(T[dtype])
+    wq, ws = quantize_i8(torch.randn(N, K, generator=g, device=DEV))
+    bias = torch.randn(N, generator=g, device=DEV)
+    q, s = quantize_i8(x)
+    L, code = _lib.lib(), {"bf16": 0, "fp16": 1, "fp32": 2}[dtype]
+    for pad, b in ((0, bias), (3, None)):
+        y = torch.full((M, N + pad), 7.0, dtype=x.dtype, device=DEV)
+        for _ in range(2):
+            _lib.check(L.lpg_fc_i8(code, M, N, K, q.data_ptr(), q.stride(0), s.data_ptr(), wq.data_ptr(), wq.stride(0),
+                                   ws.data_ptr(), None if b is None else b.data_ptr(), 1, y.data_ptr(), N + pad,
+                                   torch.cuda.current_stream().cuda_stream), "lpg_fc_i8")
+        assert pad == 0 or bool((y[:, N:] == 7.0).all())
+        for a in (0, 256 * 64 + 100, M - 512):
+            assert torch.equal(y[a:a + 512, :N], linear_i8(x[a:a + 512], wq, ws, b, relu=True))
