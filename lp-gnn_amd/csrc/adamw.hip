@@ -21,7 +21,7 @@
 // uses the moments before they are rounded.
 //
 // 67 M numbers: 277 us with fp32 moments (6.8 TB/s), 166-186 with 8-bit ones (5.8), the norm 46 (5.8); 4.2 M: 8-bit
-// step 17, norm 8 + 4; 70 K in 22 tensors 4.2 us.
+// step 17, norm 5 + 4; 70 K in 22 tensors 4.2 us.
 //
 // The norm is summed in 64 bits: products of fp32 numbers are exact there, and the sum's order does not
 // show in the 32-bit result, so the clip factor is the same however the tensors are split.
@@ -34,7 +34,10 @@ namespace {
 constexpr int kT = 256;
 constexpr int kChunk = 4096;      // elements a block
 constexpr int kChunk8 = 2048;     // ... with 8-bit moments: 67 M numbers 183 us, with 4096 190; 4.2 M 17.5 and 20.3
-constexpr int kNormChunk = 16384;  // ... of the norm (one partial sum each)
+// ... of the norm, one partial sum each: the small one up to 16 M numbers in all (4.2 M: 8.3 -> 4.8 us; of 67 M one
+// block would have to add 16000 partial sums in place of 4000)
+constexpr int kNormChunk = 16384, kNormChunkS = 4096;
+constexpr int64_t kNormSmall = (int64_t)1 << 24;
 constexpr int kQ = 256;           // elements that share a scale
 
 // Tensors a launch takes: the table is a kernel argument (at most 4 KB of them).
@@ -315,19 +318,19 @@ __device__ __forceinline__ double block_sum(double v) {
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-template <typename T>
+template <typename T, int CHUNK>
 __global__ __launch_bounds__(kT) void sumsq(TableN tab) {
-  constexpr int U = kNormChunk / (4 * kT);
+  constexpr int U = CHUNK / (4 * kT);
   const int k = tensor_of(tab);
   const lpg_tensor &e = tab.t[k];
   const T *g = static_cast<const T *>(e.p);
-  const int64_t base = (int64_t)(blockIdx.x - tab.first[k]) * kNormChunk;
+  const int64_t base = (int64_t)(blockIdx.x - tab.first[k]) * CHUNK;
   double s = 0;
   const auto add = [&](const float (&f)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) s = __builtin_fma((double)f[j], (double)f[j], s);
   };
-  if (base + kNormChunk <= e.n) {
+  if (base + CHUNK <= e.n) {
     float f[U][4];
 #pragma unroll
     for (int u = 0; u < U; ++u) {  // (ordinary loads, the step reads the gradients next: 67 M with the clip 362 -> 325 us)
@@ -363,6 +366,12 @@ __global__ __launch_bounds__(kT) void norm_scale(int64_t n, const double *__rest
 }
 
 int64_t blocks_of(int64_t n, int64_t chunk) { return (n + chunk - 1) / chunk; }
+
+int64_t norm_chunk(int64_t count, const lpg_tensor *tensors) {
+  int64_t n = 0;
+  for (int64_t i = 0; i < count && n <= kNormSmall; ++i) n += tensors[i].n;
+  return n <= kNormSmall ? kNormChunkS : kNormChunk;
+}
 
 bool hyper_ok(const lpg_adamw_hyper &h) {
   return h.beta1 >= 0.f && h.beta1 < 1.f && h.beta2 >= 0.f && h.beta2 < 1.f && h.eps >= 0.f;
@@ -441,11 +450,11 @@ extern "C" lpg_status lpg_adamw8(int32_t dtype, int64_t count, const lpg_adamw8_
 
 extern "C" int64_t lpg_grad_norm_workspace_bytes(int64_t count, const lpg_tensor *tensors) {
   if (count < 0 || (count && !tensors)) return -1;
-  int64_t blocks = 0;
-  for (int64_t i = 0; i < count; ++i) {
+  for (int64_t i = 0; i < count; ++i)
     if (tensors[i].n < 0) return -1;
-    blocks += blocks_of(tensors[i].n, kNormChunk);
-  }
+  const int64_t chunk = norm_chunk(count, tensors);
+  int64_t blocks = 0;
+  for (int64_t i = 0; i < count; ++i) blocks += blocks_of(tensors[i].n, chunk);
   return (blocks < 1 ? 1 : blocks) * (int64_t)sizeof(double);
 }
 
@@ -462,11 +471,13 @@ extern "C" lpg_status lpg_grad_norm(int32_t dtype, int64_t count, const lpg_tens
   TableN tab;
   double *part = static_cast<double *>(workspace);
   int64_t total = 0;
-  const lpg_status st = in_tables(tab, kManyN, kNormChunk, count, tensors, "lpg_grad_norm", [&](int64_t blocks) {
+  const int64_t chunk = norm_chunk(count, tensors);
+  const auto kernel = dtype == LPG_F32 ? (chunk == kNormChunk ? sumsq<float, kNormChunk> : sumsq<float, kNormChunkS>)
+                                       : (chunk == kNormChunk ? sumsq<__bf16, kNormChunk> : sumsq<__bf16, kNormChunkS>);
+  const lpg_status st = in_tables(tab, kManyN, chunk, count, tensors, "lpg_grad_norm", [&](int64_t blocks) {
     tab.part = part + total;
     total += blocks;
-    if (dtype == LPG_F32) hipLaunchKernelGGL((sumsq<float>), dim3((unsigned)blocks), dim3(kT), 0, s, tab);
-    else hipLaunchKernelGGL((sumsq<__bf16>), dim3((unsigned)blocks), dim3(kT), 0, s, tab);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kT), 0, s, tab);
   });
   if (st != LPG_OK) return st;
   hipLaunchKernelGGL(norm_scale, dim3(1), dim3(kT), 0, s, total, part, max_norm, norm, scale);
