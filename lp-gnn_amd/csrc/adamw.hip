@@ -21,7 +21,7 @@
 // uses the moments before they are rounded.
 //
 // 67 M numbers: 277 us with fp32 moments (6.8 TB/s), 166-186 with 8-bit ones (5.8), the norm 46 (5.8); 4.2 M: 8-bit
-// step 17, norm 5 + 4; 70 K in 22 tensors 4.2 us.
+// step 15, norm 5 + 4; 70 K in 22 tensors 4.2 us.
 //
 // The norm is summed in 64 bits: products of fp32 numbers are exact there, and the sum's order does not
 // show in the 32-bit result, so the clip factor is the same however the tensors are split.
@@ -32,13 +32,15 @@ namespace lpg {
 namespace {
 
 constexpr int kT = 256;
-constexpr int kChunk = 4096;      // elements a block
-constexpr int kChunk8 = 2048;     // ... with 8-bit moments: 67 M numbers 183 us, with 4096 190; 4.2 M 17.5 and 20.3
-// ... of the norm, one partial sum each: the small one up to 16 M numbers in all (4.2 M: 8.3 -> 4.8 us; of 67 M one
-// block would have to add 16000 partial sums in place of 4000)
+// Elements a block: the small chunk up to 16 M numbers in all (more waves in flight), the large one above it.  Of the
+// step with 32-bit moments, 4.2 M numbers 21.7 -> 19.0 us with the small one, 67 M 319 -> 329; of the norm (a partial sum
+// each) 4.2 M 8.3 -> 4.8, and of 67 M one block would have to add 16000 partial sums in place of 4000.  With 8-bit
+// moments 1024: 67 M 182 us, with 2048 183, 4096 190; 4.2 M 15.5, 17.7 and 20.3.
+constexpr int kChunk = 4096, kChunkS = 1024;
+constexpr int kChunk8 = 1024;
 constexpr int kNormChunk = 16384, kNormChunkS = 4096;
-constexpr int64_t kNormSmall = (int64_t)1 << 24;
-constexpr int kQ = 256;           // elements that share a scale
+constexpr int64_t kSmall = (int64_t)1 << 24;
+constexpr int kQ = 256;  // elements that share a scale
 
 // Tensors a launch takes: the table is a kernel argument (at most 4 KB of them).
 constexpr int kMany = 64, kMany8 = 56, kManyN = 128;
@@ -124,12 +126,12 @@ __device__ __forceinline__ float new_p(const lpg_adamw_hyper &h, float p, float 
   return p * h.keep - (m / (r * h.inv_root2 + h.eps)) * h.rate;
 }
 
-template <typename T>
+template <typename T, int CHUNK>
 __global__ __launch_bounds__(kT) void adamw32(Table32 tab) {
-  constexpr int U = kChunk / (4 * kT);
+  constexpr int U = CHUNK / (4 * kT);
   const int k = tensor_of(tab);
   const lpg_adamw_tensor &e = tab.t[k];
-  const int64_t base = (int64_t)(blockIdx.x - tab.first[k]) * kChunk;
+  const int64_t base = (int64_t)(blockIdx.x - tab.first[k]) * CHUNK;
   const float c = tab.scale ? *tab.scale : 1.f;
   const lpg_adamw_hyper h = tab.h;
   T *p = static_cast<T *>(e.p);
@@ -143,7 +145,7 @@ __global__ __launch_bounds__(kT) void adamw32(Table32 tab) {
       pp[j] = new_p(h, pp[j], mm[j], sqrtf(vv[j]));
     }
   };
-  if (base + kChunk <= e.n) {
+  if (base + CHUNK <= e.n) {
     float pp[U][4], gg[U][4], mm[U][4], vv[U][4];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -367,10 +369,11 @@ __global__ __launch_bounds__(kT) void norm_scale(int64_t n, const double *__rest
 
 int64_t blocks_of(int64_t n, int64_t chunk) { return (n + chunk - 1) / chunk; }
 
-int64_t norm_chunk(int64_t count, const lpg_tensor *tensors) {
+template <typename E>
+bool small(int64_t count, const E *list) {
   int64_t n = 0;
-  for (int64_t i = 0; i < count && n <= kNormSmall; ++i) n += tensors[i].n;
-  return n <= kNormSmall ? kNormChunkS : kNormChunk;
+  for (int64_t i = 0; i < count && n <= kSmall; ++i) n += list[i].n;
+  return n <= kSmall;
 }
 
 bool hyper_ok(const lpg_adamw_hyper &h) {
@@ -422,9 +425,11 @@ extern "C" lpg_status lpg_adamw(int32_t dtype, int64_t count, const lpg_adamw_te
   Table32 tab;
   tab.h = *hyper;
   tab.scale = grad_scale;
-  return in_tables(tab, kMany, kChunk, count, tensors, "lpg_adamw", [&](int64_t blocks) {
-    if (dtype == LPG_F32) hipLaunchKernelGGL((adamw32<float>), dim3((unsigned)blocks), dim3(kT), 0, s, tab);
-    else hipLaunchKernelGGL((adamw32<__bf16>), dim3((unsigned)blocks), dim3(kT), 0, s, tab);
+  const bool few = small(count, tensors);
+  const auto kernel = dtype == LPG_F32 ? (few ? adamw32<float, kChunkS> : adamw32<float, kChunk>)
+                                       : (few ? adamw32<__bf16, kChunkS> : adamw32<__bf16, kChunk>);
+  return in_tables(tab, kMany, few ? kChunkS : kChunk, count, tensors, "lpg_adamw", [&](int64_t blocks) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kT), 0, s, tab);
   });
 }
 
@@ -452,7 +457,7 @@ extern "C" int64_t lpg_grad_norm_workspace_bytes(int64_t count, const lpg_tensor
   if (count < 0 || (count && !tensors)) return -1;
   for (int64_t i = 0; i < count; ++i)
     if (tensors[i].n < 0) return -1;
-  const int64_t chunk = norm_chunk(count, tensors);
+  const int64_t chunk = small(count, tensors) ? kNormChunkS : kNormChunk;
   int64_t blocks = 0;
   for (int64_t i = 0; i < count; ++i) blocks += blocks_of(tensors[i].n, chunk);
   return (blocks < 1 ? 1 : blocks) * (int64_t)sizeof(double);
@@ -471,9 +476,10 @@ extern "C" lpg_status lpg_grad_norm(int32_t dtype, int64_t count, const lpg_tens
   TableN tab;
   double *part = static_cast<double *>(workspace);
   int64_t total = 0;
-  const int64_t chunk = norm_chunk(count, tensors);
-  const auto kernel = dtype == LPG_F32 ? (chunk == kNormChunk ? sumsq<float, kNormChunk> : sumsq<float, kNormChunkS>)
-                                       : (chunk == kNormChunk ? sumsq<__bf16, kNormChunk> : sumsq<__bf16, kNormChunkS>);
+  const bool few = small(count, tensors);
+  const auto kernel = dtype == LPG_F32 ? (few ? sumsq<float, kNormChunkS> : sumsq<float, kNormChunk>)
+                                       : (few ? sumsq<__bf16, kNormChunkS> : sumsq<__bf16, kNormChunk>);
+  const int64_t chunk = few ? kNormChunkS : kNormChunk;
   const lpg_status st = in_tables(tab, kManyN, chunk, count, tensors, "lpg_grad_norm", [&](int64_t blocks) {
     tab.part = part + total;
     total += blocks;
