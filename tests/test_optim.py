@@ -61,7 +61,9 @@ def test_c_entry_refusals():
         assert call(2, 0, None, h, None, None) == 0
     assert L.lpg_grad_norm_workspace_bytes(-1, None) == -1
     assert L.lpg_grad_norm_workspace_bytes(1, i64(p, -1)) == -1
-    assert L.lpg_grad_norm_workspace_bytes(2, i64(p, 16384, p, 16385)) == 24
+    # one fp64 sum a chunk of 4096 numbers, of 16384 above 2^24 in all
+    assert L.lpg_grad_norm_workspace_bytes(2, i64(p, 16384, p, 16385)) == 8 * (4 + 5)
+    assert L.lpg_grad_norm_workspace_bytes(2, i64(p, 2 ** 24, p, 1)) == 8 * (1024 + 1)
     assert L.lpg_grad_norm(2, 1, i64(p, 4), -1.0, p, p, p, None) == 1
     assert L.lpg_grad_norm(0, 1, i64(0, 4), 1.0, p, p, p, None) == 1
     assert L.lpg_grad_norm(2, 1, i64(p, 4), 1.0, None, p, p, None) == 1
