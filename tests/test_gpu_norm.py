@@ -287,3 +287,46 @@ def test_more_elements_than_32_bits_count():
     g, gw = torch.autograd.grad(y, (x, w), dy)
     assert torch.equal(y[-700:], small) and torch.equal(g[-700:], gs)
     assert y[:100].count_nonzero() == 0 and g[:100].count_nonzero() == 0 and gw.isfinite().all()
+
+
+def test_gradients_of_shared_and_broadcast_inputs():
+    """x, weight and bias that are expanded, strided, of more dimensions, or one tensor for both: autograd adds up
+    what the kernel gives, as with copies."""
+    from lpgnn import layer_norm
+
+    M, D = 36, 40
+    x, w, _, dy = (t.to(DEV) for t in _inputs(M, D, torch.float32, torch.float32))
+
+    def grads(make, leaves, shape=(M, D)):
+        return torch.autograd.grad(make(), leaves, dy.view(shape))
+
+    def copies(xc, wc, bc):
+        ts = [t.detach().clone().contiguous().requires_grad_(True) for t in (xc, wc, bc)]
+        return torch.autograd.grad(layer_norm(*ts, eps=EPS), ts, dy)
+
+    one = x[:1].clone().requires_grad_(True)  # every row the same one
+    base = torch.ones(D, 2, device=DEV).mul_(w[:, None]).requires_grad_(True)  # weight and bias its two columns
+    gx, gw, gb = copies(one.expand(M, D), base[:, 0], base[:, 1])
+    got = grads(lambda: layer_norm(one.expand(M, D), base[:, 0], base[:, 1], EPS), (one, base))
+    assert torch.equal(got[0], gx.sum(0, keepdim=True)) and torch.equal(got[1], torch.stack((gw, gb), 1))
+
+    xs, both = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    gx, gw, gb = copies(xs, both, both)
+    got = grads(lambda: layer_norm(xs, both, both, EPS), (xs, both))
+    assert torch.equal(got[0], gx) and torch.equal(got[1], gw + gb)
+
+    scalar = torch.full((1,), 0.7, device=DEV, requires_grad=True)
+    x3 = x.view(4, 9, D).transpose(0, 1).detach().requires_grad_(True)  # rows that no view holds
+    xp = x.view(4, 9, D).transpose(0, 1).reshape(M, D)
+    ts = [xp.clone().requires_grad_(True), scalar.detach().expand(D).clone().requires_grad_(True)]
+    want = torch.autograd.grad(layer_norm(ts[0], ts[1], None, EPS), ts, dy)
+    got = grads(lambda: layer_norm(x3, scalar.expand(D), None, EPS), (x3, scalar), (9, 4, D))
+    assert torch.equal(got[0].reshape(M, D), want[0])
+    assert abs(got[1] - want[1].double().sum()) <= D * 2.0**-24 * want[1].abs().double().sum()
+
+    v = x[0].clone().requires_grad_(True)  # one row, one dimension
+    y = layer_norm(v, w, None, EPS)
+    g, = torch.autograd.grad(y, v, dy[0])
+    r = x[:1].clone().requires_grad_(True)
+    want, = torch.autograd.grad(layer_norm(r, w, None, EPS), r, dy[:1])
+    assert y.shape == (D,) and torch.equal(g, want[0])
