@@ -93,6 +93,9 @@ int32_t code_of(at::ScalarType t) {
 // the row stride of a matrix (that of a single row says nothing)
 int64_t ld(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
+// a call's workspace on the current device: torch's allocator without a tensor around it, given back in stream order
+c10::DataPtr workspace(int64_t bytes) { return c10::GetAllocator(c10::DeviceType::CUDA)->allocate((size_t)bytes); }
+
 // t as [rows, D] with contiguous rows (a copy only where its strides allow no view)
 Tensor rows(const Tensor &t) {
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
@@ -153,17 +156,18 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const c10::DeviceGuard guard(x.device());
     const int64_t M = x.size(0), D = x.size(1);
     const Tensor dy = rows(grads[0]);
-    Tensor dx, dw, db, ws;
+    Tensor dx, dw, db;
+    c10::DataPtr ws;
     const size_t bi = w.defined() ? 2 : 1;  // (the node's edges are its tensors: one less without a weight)
     if (ctx->needs_input_grad(0)) dx = at::empty({M, D}, x.options());
     if (w.defined() && ctx->needs_input_grad(1)) dw = at::empty({D}, w.options());
     if (b.defined() && ctx->needs_input_grad(bi)) db = at::empty({D}, b.options());
     if (dw.defined() || db.defined())
-      ws = at::empty({L.layer_norm_bwd_workspace_bytes(M, D) / 4}, x.options().dtype(at::kFloat));
+      ws = workspace(L.layer_norm_bwd_workspace_bytes(M, D));
     const float *mean = stats.data_ptr<float>();
     check(L.layer_norm_bwd(code_of(x.scalar_type()), weight_code(w, b), M, D, x.data_ptr(), ld(x), dy.data_ptr(),
                            ld(dy), ptr(w), ptr(b), mean, mean + M,
-                           ctx->saved_data["relu"].toBool() ? LPG_NORM_RELU : 0, ptr(dx), D, ptr(dw), ptr(db), ptr(ws),
+                           ctx->saved_data["relu"].toBool() ? LPG_NORM_RELU : 0, ptr(dx), D, ptr(dw), ptr(db), ws.get(),
                            stream_of(x)),
           "lpg_layer_norm_bwd");
     if (at::GradMode::is_enabled()) {
@@ -392,9 +396,9 @@ std::pair<Tensor, Tensor> clip_scale(handle grads, double max_norm) {
   const c10::DeviceGuard guard(gs[0].device());
   const auto f32 = gs[0].options().dtype(at::kFloat);
   Tensor norm = at::empty({}, f32), scale = at::empty({}, f32);
-  Tensor ws = at::empty({L.grad_norm_workspace_bytes((int64_t)tab.size(), tab.data()) / 8}, f32.dtype(at::kDouble));
+  const c10::DataPtr ws = workspace(L.grad_norm_workspace_bytes((int64_t)tab.size(), tab.data()));
   check(L.grad_norm(type, (int64_t)tab.size(), tab.data(), max_norm, norm.data_ptr<float>(), scale.data_ptr<float>(),
-                    ws.data_ptr(), stream_of(norm)),
+                    ws.get(), stream_of(norm)),
         "lpg_grad_norm");
   return {norm, scale};
 }
@@ -481,11 +485,13 @@ Tensor linear_i8(const Tensor &x, const Tensor &wq, const Tensor &ws, const OptT
   }
   if (M > 0) {
     const int64_t rows = L.i8_chunk_rows(M, N, K), most = rows < M ? rows + rows / 4 : M, ldq = code_pitch(a, b);
-    Tensor q = at::empty({most, ldq}, a.options().dtype(at::kChar)), s = at::empty({most}, a.options().dtype(at::kFloat));
+    const c10::DataPtr codes = workspace(most * ldq), scales = workspace(most * 4);
+    int8_t *const q = static_cast<int8_t *>(codes.get());
+    float *const s = static_cast<float *>(scales.get());
     for (int64_t at = 0, m; at < M; at += m) {
       m = std::min(L.i8_chunk_rows(M - at, N, K), most);
-      quant(a, b, at, m, ptr_of<int8_t>(q), ldq, ptr_of<float>(s));
-      check(L.fc_i8(type, m, N, K, ptr_of<int8_t>(q), ldq, ptr_of<float>(s), ptr_of<int8_t>(w), ldw, ptr_of<float>(scale),
+      quant(a, b, at, m, q, ldq, s);
+      check(L.fc_i8(type, m, N, K, q, ldq, s, ptr_of<int8_t>(w), ldw, ptr_of<float>(scale),
                     ptr_of<float>(bb), flags, static_cast<char *>(y.data_ptr()) + at * N * y.element_size(), N,
                     stream_of(x)),
             "lpg_fc_i8");
