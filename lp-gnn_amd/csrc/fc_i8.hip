@@ -187,11 +187,11 @@ __device__ __forceinline__ void part_quant(const T *p, int n, int t, int nt, con
   }
 }
 
-// zeros from q[k] to q[end], end a multiple of 4, by lanes l of G
+// zeros from q[k] to q[end], q and end multiples of 16, by lanes l of G
 __device__ __forceinline__ void zero_from(int8_t *q, int k, int end, int l, int G) {
-  const int k4 = (k + 3) & ~3;
-  for (int i = k + l; i < k4; i += G) q[i] = 0;
-  for (int i = k4 + l * 4; i < end; i += G * 4) *reinterpret_cast<uint32_t *>(q + i) = 0;
+  const int k16 = (k + 15) & ~15;
+  for (int i = k + l; i < k16; i += G) q[i] = 0;
+  for (int i = k16 + l * 16; i < end; i += G * 16) *reinterpret_cast<u32x4 *>(q + i) = u32x4{0u, 0u, 0u, 0u};
 }
 
 struct QuantArgs {
@@ -220,20 +220,24 @@ __global__ __launch_bounds__(256) void quant_rows(QuantArgs a) {
 }
 
 // A row of at most G NV vectors, held in the registers of G lanes: all its loads in flight together, read once.
-// Vector i of the row is a vector of x or, from K1 / V on, of x2; the columns that fill no vector (2 V - 2 at
-// most) are single elements of the lanes.
-template <typename T, int G, int NV>
+// Vector i of the row is a vector of x or, from n1 on, of x2; where the columns are no multiple of V the last one
+// starts early, to end with them (the elements it shares with the one before get the same codes twice).  REST: the
+// columns that fill no vector (2 V - 2 at most) are single elements of the lanes instead, for K1 or K2 below V.
+template <typename T, int G, int NV, bool REST>
 struct HeldRow {
-  static constexpr int V = 16 / sizeof(T), NR = (2 * V - 2 + G - 1) / G;
+  static constexpr int V = 16 / sizeof(T), NR = REST ? (2 * V - 2 + G - 1) / G : 0;
   u32x4 v[NV];
-  float rest[NR];
+  float rest[NR ? NR : 1];
+  static __device__ __forceinline__ int count(int K) { return REST ? K / V : (K + V - 1) / V; }
+  // where vector i of K columns starts
+  static __device__ __forceinline__ int start(int i, int K) { return REST || i * V + V <= K ? i * V : K - V; }
   __device__ __forceinline__ void load(const T *x, int K1, const T *x2, int K2, int l) {
-    const int n1 = K1 / V, n2 = K2 / V, r1 = K1 % V, r2 = K2 % V;
+    const int n1 = count(K1), n2 = count(K2), r1 = K1 % V, r2 = K2 % V;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int i = k * G + l;
       v[k] = u32x4{0u, 0u, 0u, 0u};
-      if (i < n1 + n2) __builtin_memcpy(&v[k], i < n1 ? x + i * V : x2 + (i - n1) * V, 16);
+      if (i < n1 + n2) __builtin_memcpy(&v[k], i < n1 ? x + start(i, K1) : x2 + start(i - n1, K2), 16);
     }
 #pragma unroll
     for (int k = 0; k < NR; ++k) {
@@ -251,7 +255,7 @@ struct HeldRow {
     return lanes_max<G>(m);
   }
   __device__ __forceinline__ void store(const RowScale &s, int8_t *q, int K1, int K2, int l) const {
-    const int n1 = K1 / V, n2 = K2 / V, r1 = K1 % V, r2 = K2 % V;
+    const int n1 = count(K1), n2 = count(K2), r1 = K1 % V, r2 = K2 % V;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int i = k * G + l;
@@ -260,7 +264,7 @@ struct HeldRow {
       uint32_t o[V / 4];
       unpack<T>(v[k], f);
       quant<V>(f, s, o);
-      __builtin_memcpy(q + (i < n1 ? i * V : K1 + (i - n1) * V), o, V);
+      __builtin_memcpy(q + (i < n1 ? start(i, K1) : K1 + start(i - n1, K2)), o, V);
     }
 #pragma unroll
     for (int k = 0; k < NR; ++k) {
@@ -275,11 +279,11 @@ struct HeldRow {
   }
 };
 
-template <typename T, int G, int NV>
+template <typename T, int G, int NV, bool REST = false>
 __global__ __launch_bounds__(256) void quant_rows_held(QuantArgs a) {
   const int l = threadIdx.x % G;
   const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, at = row < a.M ? row : a.M - 1;
-  HeldRow<T, G, NV> h;
+  HeldRow<T, G, NV, REST> h;
   h.load(static_cast<const T *>(a.x) + at * a.ldx, a.K1, a.K2 ? static_cast<const T *>(a.x2) + at * a.ldx2 : nullptr,
          a.K2, l);
   const RowScale s(h.top());  // (of every lane: rows past the end are the last one again)
@@ -645,7 +649,7 @@ __global__ __launch_bounds__(512) void fc_i8_some(RowsArgs a) {
   const int pitch = ks * 64 + 16;  // (rows 16 bytes apart in the banks)
   const int64_t m0 = (int64_t)blockIdx.y * 16, n0 = (int64_t)blockIdx.x * kSomeN + wave * 16;
   const int fr = lane & 15, fq = lane >> 4;
-  HeldRow<T, 64, NV> h[2];
+  HeldRow<T, 64, NV, true> h[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int64_t row = m0 + wave * 2 + i < a.M ? m0 + wave * 2 + i : a.M - 1;
@@ -833,18 +837,27 @@ extern "C" lpg_status lpg_quant_i8(int32_t dtype, int64_t M, int64_t K1, const v
     LPG_HIP(hipGetLastError());
     return LPG_OK;
   };
-  // the fewest lanes, from 8 on, that hold a row in one vector each, else a wave and up to 16 vectors a lane (100 K
-  // rows of 100 fp16 numbers: 43 us with a wave a row, 15 with 16 lanes); longer rows are read twice
+  // The fewest lanes, from 8 on, that hold a row in up to four vectors each, else a wave and up to 16 vectors a lane:
+  // what a row costs beside its elements (its largest, two divisions) is shared by as many rows of the wave as it holds
+  // (700 K x 300 bf16: 340 us with a vector a lane and 64 lanes, 142 with three and 16; 1.6 M x 128 179 and 124).  Two
+  // or four lanes cost more than they share (2.1 M x 100 155 us with eight, 211 with four); the shortest rows are faster
+  // with a vector a lane (3.3 M x 64 163 us, two lanes of four 264); longer rows than 16 vectors a lane are read twice.
   const auto of = [&](auto t) -> lpg_status {
     using T = decltype(t);
     constexpr int V = 16 / sizeof(T);
-    const int64_t n = K1 / V + K2 / V;
-    if (n <= 8) return go(quant_rows_held<T, 8, 1>, 32);
-    if (n <= 16) return go(quant_rows_held<T, 16, 1>, 16);
-    if (n <= 32) return go(quant_rows_held<T, 32, 1>, 8);
-    if (n <= 64) return go(quant_rows_held<T, 64, 1>, 4);
-    if (n <= 128) return go(quant_rows_held<T, 64, 2>, 4);
+    if (K1 / V + K2 / V <= 8) return go(quant_rows_held<T, 8, 1, true>, 32);
+    if (K1 < V || (K2 > 0 && K2 < V)) return go(quant_rows<T>, 4);  // (a part without a vector, beside a long one)
+    const int64_t n = (K1 + V - 1) / V + (K2 + V - 1) / V;
+    if (n <= 16) return go(quant_rows_held<T, 8, 2>, 32);
+    if (n <= 24) return go(quant_rows_held<T, 8, 3>, 32);
+    if (n <= 32) return go(quant_rows_held<T, 8, 4>, 32);
+    if (n <= 48) return go(quant_rows_held<T, 16, 3>, 16);
+    if (n <= 64) return go(quant_rows_held<T, 16, 4>, 16);
+    if (n <= 96) return go(quant_rows_held<T, 32, 3>, 8);
+    if (n <= 128) return go(quant_rows_held<T, 32, 4>, 8);
+    if (n <= 192) return go(quant_rows_held<T, 64, 3>, 4);
     if (n <= 256) return go(quant_rows_held<T, 64, 4>, 4);
+    if (n <= 384) return go(quant_rows_held<T, 64, 6>, 4);
     if (n <= 512) return go(quant_rows_held<T, 64, 8>, 4);
     if (n <= 1024) return go(quant_rows_held<T, 64, 16>, 4);
     return go(quant_rows<T>, 4);

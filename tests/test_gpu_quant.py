@@ -257,3 +257,23 @@ def test_blocks_that_go_on_to_further_tiles(M, N, K, dtype):
         assert pad == 0 or bool((y[:, N:] == 7.0).all())
         for a in (0, 256 * 64 + 100, M - 512):
             assert torch.equal(y[a:a + 512, :N], linear_i8(x[a:a + 512], wq, ws, b, relu=True))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("K1,K2", [(65, 0), (70, 3), (90, 45), (97, 7), (150, 150), (200, 8), (300, 0), (301, 299),
+                                   (5, 700), (760, 2), (1030, 0), (777, 778), (1537, 0), (2500, 33), (3, 2050),
+                                   (4097, 0), (8000, 193)])
+def test_codes_of_every_row_length(K1, K2, dtype):
+    """The rows' codes where the last vectors overlap, parts are shorter than a vector and lanes run out; the
+    padding is zero, rows beside each other are left alone."""
+    from lpgnn import quantize_i8
+
+    M = 67
+    x, x2, _, _ = _case(M, 1, K1, K2, T[dtype], seed=3)
+    wide = torch.full((M, K1 + 3), float("nan"), dtype=x.dtype, device=DEV)
+    wide[:, 1:1 + K1] = x.to(DEV)
+    q, s = quantize_i8(wide[:, 1:1 + K1], _dev(x2))
+    want, ws, _ = R.quantize(x if x2 is None else torch.cat((x, x2), 1))
+    assert torch.equal(q.cpu().to(want.dtype), want) and torch.equal(s.cpu(), ws.view(-1).to(s.dtype))
+    pitch = q.stride(0)
+    assert not q.as_strided((M, pitch), (pitch, 1))[:, K1 + K2:].any()
