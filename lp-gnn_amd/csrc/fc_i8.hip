@@ -149,6 +149,18 @@ __device__ __forceinline__ void unpack(u32x4 v, float (&f)[16 / sizeof(T)]) {
   for (int j = 0; j < (int)(16 / sizeof(T)); ++j) f[j] = (float)t[j];
 }
 
+// 16 bytes at any element alignment, past the caches or through them
+typedef unsigned int u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+template <bool PAST, typename T>
+__device__ __forceinline__ u32x4 ld16(const T *p) {
+  u32x4 v;
+  if constexpr (PAST)
+    v = __builtin_nontemporal_load(reinterpret_cast<const std::conditional_t<sizeof(T) == 2, u32x4_at2, u32x4_at4> *>(p));
+  else __builtin_memcpy(&v, p, 16);
+  return v;
+}
+
 // the largest |x| bits of the n elements at p, taken by threads t of nt
 template <typename T>
 __device__ __forceinline__ uint32_t part_max(const T *p, int n, int t, int nt) {
@@ -200,6 +212,7 @@ struct QuantArgs {
   const void *x, *x2;
   int8_t *q;
   float *scale;
+  int past;  // x is read past the caches
 };
 
 template <typename T>
@@ -231,13 +244,14 @@ struct HeldRow {
   static __device__ __forceinline__ int count(int K) { return REST ? K / V : (K + V - 1) / V; }
   // where vector i of K columns starts
   static __device__ __forceinline__ int start(int i, int K) { return REST || i * V + V <= K ? i * V : K - V; }
+  template <bool PAST = false>
   __device__ __forceinline__ void load(const T *x, int K1, const T *x2, int K2, int l) {
     const int n1 = count(K1), n2 = count(K2), r1 = K1 % V, r2 = K2 % V;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int i = k * G + l;
       v[k] = u32x4{0u, 0u, 0u, 0u};
-      if (i < n1 + n2) __builtin_memcpy(&v[k], i < n1 ? x + start(i, K1) : x2 + start(i - n1, K2), 16);
+      if (i < n1 + n2) v[k] = ld16<PAST>(i < n1 ? x + start(i, K1) : x2 + start(i - n1, K2));
     }
 #pragma unroll
     for (int k = 0; k < NR; ++k) {
@@ -284,8 +298,9 @@ __global__ __launch_bounds__(256) void quant_rows_held(QuantArgs a) {
   const int l = threadIdx.x % G;
   const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, at = row < a.M ? row : a.M - 1;
   HeldRow<T, G, NV, REST> h;
-  h.load(static_cast<const T *>(a.x) + at * a.ldx, a.K1, a.K2 ? static_cast<const T *>(a.x2) + at * a.ldx2 : nullptr,
-         a.K2, l);
+  const T *x = static_cast<const T *>(a.x) + at * a.ldx, *x2 = a.K2 ? static_cast<const T *>(a.x2) + at * a.ldx2 : nullptr;
+  if (a.past) h.template load<true>(x, a.K1, x2, a.K2, l);
+  else h.load(x, a.K1, x2, a.K2, l);
   const RowScale s(h.top());  // (of every lane: rows past the end are the last one again)
   if (row >= a.M) return;
   int8_t *q = a.q + row * a.ldq;
@@ -830,7 +845,10 @@ extern "C" lpg_status lpg_quant_i8(int32_t dtype, int64_t M, int64_t K1, const v
   LPG_REQUIRE(M == 0 || (x && q && scale && (K2 == 0 || x2)), "lpg_quant_i8: NULL pointer");
   LPG_REQUIRE(aligned16(q), "lpg_quant_i8: q must be 16-byte aligned");
   LPG_REQUIRE((M + 3) / 4 <= INT32_MAX, "lpg_quant_i8: too many rows");
-  const QuantArgs a{M, ldx, ldx2, ldq, (int)K1, (int)K2, x, x2, q, scale};
+  // x past the caches where it would push out the codes (100 K x 2048 fp32 with the product to 1024 469 -> 394 us, 60 K x
+  // 2048 fp16 187 -> 177); a small x may still be in them (20000 x 1024 fp16 45 us through them, 47 past them)
+  const int past = M * (K1 + K2) * (dtype == LPG_F32 ? 4 : 2) > (int64_t)128 << 20;
+  const QuantArgs a{M, ldx, ldx2, ldq, (int)K1, (int)K2, x, x2, q, scale, past};
   const auto go = [&](auto kernel, int rows) -> lpg_status {
     if (M == 0) return LPG_OK;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((M + rows - 1) / rows)), dim3(256), 0, as_stream(stream), a);
