@@ -16,7 +16,7 @@
 // bytes: 128-byte k tiles staged by buffer_load ... lds into a swizzled image, two buffers (four in the small tile),
 // one barrier a tile in its middle, fragment reads one half tile ahead, transposed fragments (W x A^T: a lane holds
 // four consecutive columns of one row), stores straight from registers.  16384 x 2048, K = 4096: 108 us, 2.55 POPS;
-// 100 K x 1024, K = 2048: 194 us, 2.16 (a k tile takes 1.4 us, of which the MFMAs 0.85 at 2.4 GHz; the first round's
+// 100 K x 1024, K = 2048: 194 us, 2.16 (170 behind the codes in cache; a k tile takes 1.4 us, of which the MFMAs 0.85 at 2.4 GHz; the first round's
 // loads and the last one's stores are not hidden).
 // fc_i8_row, fc_i8_some: few rows are bound by latency -- the second launch, the k loop's barriers -- and by
 // w's bytes: every block quantises its rows into LDS itself, its first loads of w in flight meanwhile.  One row of
@@ -536,7 +536,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fc_i8(FcArgs a) {
       for (int r = 0; r < 4; ++r) ws[j][r] = cs[j * 16 + r], bb[j][r] = cb[j * 16 + r];
     // all stores of the wave's part: of a whole tile past the caches or through them, or whatever exists of it
     const auto store = [&](auto how) {
-      constexpr bool WHOLE = decltype(how)::value < 2, PAST = decltype(how)::value == 0;  // (PAST: of 16 bits)
+      constexpr bool WHOLE = decltype(how)::value < 2, PAST = decltype(how)::value == 0;
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         const int64_t row = r0 + i * 16 + er;
@@ -548,7 +548,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fc_i8(FcArgs a) {
             const int64_t c = c0 + j * 16 + eq * 4;
             const float out[4] = {v(j, 0), v(j, 1), v(j, 2), v(j, 3)};
             T *p = y + row * a.ldy + c;
-            if (WHOLE || (row < a.M && c + 4 <= a.N)) {
+            if constexpr (PAST) {
+              u32x4 o;
+              __builtin_memcpy(&o, out, 16);
+              __builtin_nontemporal_store(o, reinterpret_cast<u32x4 *>(p));
+            } else if (WHOLE || (row < a.M && c + 4 <= a.N)) {
               __builtin_memcpy(p, out, 16);
             } else if (row < a.M && c < a.N) {
 #pragma unroll
@@ -589,7 +593,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fc_i8(FcArgs a) {
         }
       }
     };
-    if (sizeof(T) == 2 && stored && a.past) store(std::integral_constant<int, 0>());
+    if (stored && a.past) store(std::integral_constant<int, 0>());
     else if (stored) store(std::integral_constant<int, 1>());
     else store(std::integral_constant<int, 2>());
     if constexpr (!ON) break;
@@ -823,14 +827,14 @@ using namespace lpg;
     return LPG_ERR_INVALID;                                                              \
   } while (0)
 
-// 96 MiB of codes: written by the one kernel and read by the other they stay in the 256 MiB of last-level cache
-// beside w and the streams of x and y.  Whole rounds of 256-row tiles, and up to a quarter more in place of a short
-// last chunk.  200 K x 2048, K = 4096 with 48 / 64 / 96 / 128 MiB 2.03 / 1.86 / 1.83 / 1.92 ms, 200 K x 1024, K = 2048
-// 0.64 / 0.61 / 0.59 / 0.67; half a chunk more instead of a quarter: 130 K x 1024, K = 1024 0.257 against 0.220.
+// 160 MiB of codes: written by the one kernel and read by the other they stay in the 256 MiB of last-level cache (the
+// streams of large x and y go past it).  Whole rounds of 256-row tiles, and up to a quarter more in place of a short
+// last chunk.  200 K x 2048, K = 4096 bf16 with 64 / 96 / 160 / 192 MiB 1.83 / 1.72 / 1.66 / 1.64 ms, 150 K x 1500, K =
+// 3000 fp16 0.95 / 0.81 / 0.80 / 0.85; half a chunk more instead of a quarter: 130 K x 1024, K = 1024 0.257 against 0.220.
 extern "C" int64_t lpg_i8_chunk_rows(int64_t M, int64_t N, int64_t K) {
   if (M < 0 || N < 1 || K < 1) return -1;
   const int64_t ldq = (K + 127) / 128 * 128, nt = (N + 255) / 256, cus = device_cus();
-  const int64_t rounds = ((int64_t)96 << 20) / ldq / 256 * nt / cus;
+  const int64_t rounds = ((int64_t)160 << 20) / ldq / 256 * nt / cus;
   int64_t rows = (rounds < 1 ? 1 : rounds) * cus / nt * 256;
   rows = rows < 256 ? 256 : rows;
   return M < rows + rows / 4 ? M : rows;
@@ -897,10 +901,11 @@ extern "C" lpg_status lpg_fc_i8(int32_t dtype, int64_t M, int64_t N, int64_t K, 
   LPG_REQUIRE(aligned16(q) && aligned16(w), "lpg_fc_i8: q and w must be 16-byte aligned");
   LPG_REQUIRE(((M + 63) / 64) <= INT32_MAX / ((N + 63) / 64), "lpg_fc_i8: too many tiles");
   // Past the caches go outputs that would push out the codes: not short sums' (100 K x 1024, K = 64 60 us through
-  // them, 73 past them), not small ones (20000 x 1024, K = 1024 41 and 43; 200 K x 2048, K = 1024 629 and 537), only
-  // rows on whole lines (30000 x 1000, K = 2000 62 us through them, 86 past them), not fp32's (their stores take
-  // longer than the codes: 100 K x 512, K = 256 83 and 99).
-  const int past = dtype != LPG_F32 && K > 128 && M * N > (int64_t)32 << 20 && ldy % 64 == 0 &&
+  // them, 73 past them; fp32 100 K x 512, K = 512 95 and 117, x 1024, K = 1024 251 and 226), not small ones (20000 x
+  // 1024, K = 1024 41 and 43; 200 K x 2048, K = 1024 629 and 537), only rows on whole lines (30000 x 1000, K = 2000 62 us
+  // through them, 86 past them).
+  const int64_t e = dtype == LPG_F32 ? 4 : 2;
+  const int past = K > (e == 4 ? 512 : 128) && M * N * e > (int64_t)64 << 20 && ldy * e % 128 == 0 &&
                    reinterpret_cast<uintptr_t>(y) % 128 == 0;
   const FcArgs a{M, N, ldq, ldw, ldy, (int)K, q, w, scale, wscale, bias, y, 0, 0,
                  (flags & LPG_FC_RELU) ? 0.f : -INFINITY, past};

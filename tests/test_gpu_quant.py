@@ -236,7 +236,8 @@ def test_more_elements_than_32_bits_count():
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("M,N,K", [(256 * 150 + 5, 512, 100), (256 * 150, 512, 129), (256 * 280, 512, 260),
-                                   (300 * 128 + 1, 1100, 40), (256 * 131, 1024, 384)])
+                                   (300 * 128 + 1, 1100, 40), (256 * 131, 1024, 384),
+                                   (256 * 132, 1024, 600)])
 def test_blocks_that_go_on_to_further_tiles(M, N, K, dtype):
     """More tiles than blocks, of one k tile and of several, whole ones and cut ones, outputs on lines and off: the
     codes' product by the C entry is that of few rows at a time."""
