@@ -16,8 +16,8 @@
 // bytes: 128-byte k tiles staged by buffer_load ... lds into a swizzled image, two buffers (four in the small tile),
 // one barrier a tile in its middle, fragment reads one half tile ahead, transposed fragments (W x A^T: a lane holds
 // four consecutive columns of one row), stores straight from registers.  16384 x 2048, K = 4096: 108 us, 2.55 POPS;
-// 100 K x 1024, K = 2048: 194 us, 2.16 (170 behind the codes in cache; a k tile takes 1.4 us, of which the MFMAs 0.85 at 2.4 GHz; the first round's
-// loads and the last one's stores are not hidden).
+// 100 K x 1024, K = 2048: 194 us, 2.16, and 170 behind the codes (in cache then).  A k tile takes 1.4 us, of which the
+// MFMAs 0.85 at 2.4 GHz; the first round's loads and the last one's stores are not hidden.
 // fc_i8_row, fc_i8_some: few rows are bound by latency -- the second launch, the k loop's barriers -- and by
 // w's bytes: every block quantises its rows into LDS itself, its first loads of w in flight meanwhile.  One row of
 // 2048 to 1024 columns: 3.8 us.
