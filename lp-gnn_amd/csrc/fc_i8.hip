@@ -527,7 +527,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fc_i8(FcArgs a) {
     origin(tile, m0, n0);
     stored = m0 + BM <= a.M && n0 + BN <= a.N;
     const int64_t r0 = m0 + wm * FM * 16, c0 = n0 + wn * FN * 16;
-    const float *rs = sc + scales * SC + wm * FM * 16 + er, *cs = sc + scales * SC + BM + wn * FN * 16 + eq * 4, *cb = cs + BN;
+    const float *rs = sc + scales * SC + wm * FM * 16 + er;
+    const float *cs = sc + scales * SC + BM + wn * FN * 16 + eq * 4, *cb = cs + BN;
     scales = scales + 1 < NS ? scales + 1 : 0;
     float ws[FN][4], bb[FN][4];
 #pragma unroll
@@ -576,7 +577,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fc_i8(FcArgs a) {
               out[2 + d] = z[1];
             }
             const int64_t c = c0 + j * 16 + eq * 8;
-            __builtin_amdgcn_sched_barrier(0);  // (a store as soon as its numbers are: 16384 x 1024, K = 128 14.8 -> 12.9 us)
+            // (a store as soon as its numbers are: 16384 x 1024, K = 128 14.8 -> 12.9 us)
+            __builtin_amdgcn_sched_barrier(0);
             T *p = y + row * a.ldy + c;
             if constexpr (PAST) {
               __builtin_nontemporal_store(out, reinterpret_cast<u32x4 *>(p));
@@ -930,7 +932,8 @@ extern "C" lpg_status lpg_fc_i8_rows(int32_t dtype, int64_t M, int64_t N, int64_
     set_error("lpg_fc_i8_rows: too many or too long rows for one launch (use lpg_quant_i8 and lpg_fc_i8)");
     return LPG_ERR_UNSUPPORTED;
   }
-  const RowsArgs a{M, N, ldx, ldx2, ldw, ldy, (int)K1, (int)K2, x, x2, w, wscale, bias, y, (flags & LPG_FC_RELU) ? 0.f : -INFINITY};
+  const RowsArgs a{M, N, ldx, ldx2, ldw, ldy, (int)K1, (int)K2, x, x2, w, wscale, bias, y,
+                   (flags & LPG_FC_RELU) ? 0.f : -INFINITY};
 #define F(T) M == 0 ? LPG_OK : run_rows<T>(a, as_stream(stream))
   LPG_I8_TYPES("lpg_fc_i8_rows", F);
 #undef F

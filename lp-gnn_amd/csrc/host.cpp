@@ -378,8 +378,9 @@ void adamw_step_8bit(handle params_, handle grads, handle m8_, handle m_scales, 
   apart(what, gs, {&ps, &m8, &ms, &r8, &rs});
   std::vector<lpg_adamw8_tensor> tab(ps.size());
   for (size_t i = 0; i < ps.size(); ++i)
-    tab[i] = {ps[i].data_ptr(),      gs[i].data_ptr(), m8[i].data_ptr(), ptr_of<float>(ms[i]),
-              r8[i].data_ptr(), ptr_of<float>(rs[i]), ps[i].numel(),    rounding_key(places ? (*places)[i] : (int64_t)i, step, seed)};
+    tab[i] = {ps[i].data_ptr(), gs[i].data_ptr(),      m8[i].data_ptr(), ptr_of<float>(ms[i]),
+              r8[i].data_ptr(), ptr_of<float>(rs[i]), ps[i].numel(),
+              rounding_key(places ? (*places)[i] : (int64_t)i, step, seed)};
   const c10::DeviceGuard guard(ps[0].device());
   check(L.adamw8(type, (int64_t)tab.size(), tab.data(), &h, scale, stream_of(ps[0])), "lpg_adamw8");
   written(ps), written(m8), written(ms), written(r8), written(rs);
@@ -465,7 +466,8 @@ Tensor linear_i8(const Tensor &x, const Tensor &wq, const Tensor &ws, const OptT
   const int64_t k16 = (K + 15) / 16 * 16;
   int64_t ldw = N > 1 ? w.stride(0) : k16;
   const bool room = (w.storage_offset() + (N - 1) * ldw + k16) <= (int64_t)w.storage().nbytes();
-  if ((w.stride(1) != 1 && K > 1) || ldw < k16 || ldw % 16 || ldw > (1 << 22) || !room || reinterpret_cast<uintptr_t>(w.data_ptr()) % 16) {
+  if ((w.stride(1) != 1 && K > 1) || ldw < k16 || ldw % 16 || ldw > (1 << 22) || !room ||
+      reinterpret_cast<uintptr_t>(w.data_ptr()) % 16) {
     w = at::empty({N, k16}, wq.options()).narrow(1, 0, K);
     w.copy_(wq);
     ldw = k16;

@@ -453,3 +453,27 @@ def test_more_elements_than_32_bits_count(bits):
             a, b = a[-k:].float(), b.float()
             assert ((a - b).abs() <= torch.maximum(a.abs(), b.abs()) / 8 + 2.0**-9).all() and a.count_nonzero() > k // 2
     assert torch.equal(p[-k:], p0) and p[:1000].count_nonzero() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_split_over_blocks_does_not_show(dtype):
+    """More numbers than the small chunks are for, in one call and in pieces of it: the same bits, and the norm of all
+    is the pieces' together."""
+    from lpgnn import optim
+
+    n = 2**24 + 4099
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    r = lambda: torch.randn(n, generator=gen, device=DEV)
+    p, g, m, v = r().to(dtype), r().to(dtype), r(), r().square()
+    pieces = [0, 5, 2**20 + 3, 2**23, n]
+    a = [t.clone() for t in (p, g, m, v)]
+    optim.adamw_step(*[[t] for t in a], step=7, **H)
+    for lo, hi in zip(pieces, pieces[1:]):
+        optim.adamw_step(*[[t[lo:hi]] for t in (p, g, m, v)], step=7, **H)
+    assert all(torch.equal(x, y) for x, y in zip(a, (p, g, m, v)))
+    whole, scale = optim.clip_scale([g], 0.5)
+    cut, scale2 = optim.clip_scale([g[lo:hi] for lo, hi in zip(pieces, pieces[1:])], 0.5)
+    want = g.double().square().sum().sqrt()
+    for x in (whole, cut):
+        assert abs(x.double() - want) <= (2.0**-24 + n * 2.0**-53) * want
+    assert abs(scale - scale2) <= 2.0**-22 * scale
