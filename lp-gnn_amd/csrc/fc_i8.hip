@@ -798,8 +798,8 @@ lpg_status run_rows(const RowsArgs &a, hipStream_t s) {
     };
     if (nv <= 1) go(fc_i8_some<T, 1>);
     else if (nv <= 2) go(fc_i8_some<T, 2>);
-    else if (nv <= 4) go(fc_i8_some<T, 4>);
-    else go(fc_i8_some<T, 8>);  // (fp32)
+    else if (nv <= 4 || sizeof(T) == 2) go(fc_i8_some<T, 4>);  // (16 bits: at most 160 vectors)
+    else if constexpr (sizeof(T) == 4) go(fc_i8_some<T, 5>);   // (at most 320)
   }
   LPG_HIP(hipGetLastError());
   return LPG_OK;
