@@ -278,3 +278,22 @@ def test_codes_of_every_row_length(K1, K2, dtype):
     assert torch.equal(q.cpu().to(want.dtype), want) and torch.equal(s.cpu(), ws.view(-1).to(s.dtype))
     pitch = q.stride(0)
     assert not q.as_strided((M, pitch), (pitch, 1))[:, K1 + K2:].any()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 3, 5000), (3, 1, 40), (700, 1, 1281), (9000, 1, 33), (9000, 2, 200),
+                                   (33000, 17, 64), (50, 129, 1280), (50, 129, 1281), (20000, 255, 129)])
+def test_smallest_sides(M, N, K):
+    """One column, one row, one number; both sides of the longest row that few rows take in one launch."""
+    for dtype in (torch.float16, torch.float32):
+        x, _, W, bias = _case(M, N, K, 0, dtype, seed=5)
+        _check(x, None, W, bias, True)
+
+
+def test_one_tensor_as_both_parts():
+    from lpgnn import linear_i8, quantize_i8
+
+    x, _, W, bias = _case(70, 40, 24, 0, torch.bfloat16)
+    xd, wq, ws = _dev(x), *quantize_i8(_dev(torch.cat((W, W), 1)))
+    assert torch.equal(linear_i8(xd, wq, ws, _dev(bias), x2=xd), linear_i8(xd.repeat(1, 2), wq, ws, _dev(bias)))
+    rows = xd[:1].expand(70, 24)  # a broadcast input
+    assert torch.equal(linear_i8(rows, wq, ws, x2=rows), linear_i8(rows.contiguous(), wq, ws, x2=rows.contiguous()))
