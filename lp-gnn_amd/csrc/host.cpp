@@ -96,6 +96,15 @@ int64_t ld(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 // a call's workspace on the current device: torch's allocator without a tensor around it, given back in stream order
 c10::DataPtr workspace(int64_t bytes) { return c10::GetAllocator(c10::DeviceType::CUDA)->allocate((size_t)bytes); }
 
+// The operators have no forward-mode derivative: a dual tensor's tangent would be dropped, which reads as a derivative
+// of zero.
+void no_tangent(const char *what, const Tensor &t) {
+  REQUIRE(!t.defined() || !t._fw_grad(0).defined(), "lpgnn ", what, ": there is no forward-mode derivative");
+}
+void no_tangent(const char *what, const OptTensor &t) {
+  if (t) no_tangent(what, *t);
+}
+
 // t as [rows, D] with contiguous rows (a copy only where its strides allow no view)
 Tensor rows(const Tensor &t) {
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
@@ -181,6 +190,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double eps, bool relu) {
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  for (const Tensor *t : {&x, &w, &b}) no_tangent("layer_norm", *t);
   REQUIRE(x.is_cuda(), "lpgnn layer_norm: runs on a HIP device only (no CPU path)");
   REQUIRE(code_of(x.scalar_type()) >= 0, "lpgnn layer_norm: x must be float32, bfloat16 or float16, got ",
           x.scalar_type());
@@ -230,8 +240,10 @@ struct Tensors {
     if (!fast) throw pybind11::error_already_set();
     n = (size_t)PySequence_Fast_GET_SIZE(fast.ptr());
     items = PySequence_Fast_ITEMS(fast.ptr());
-    for (size_t i = 0; i < n; ++i)
+    for (size_t i = 0; i < n; ++i) {
       if (!THPVariable_Check(items[i])) throw pybind11::type_error(c10::str("lpgnn ", what, ": the lists hold tensors"));
+      no_tangent(what, (*this)[i]);
+    }
   }
   size_t size() const { return n; }
   bool empty() const { return n == 0; }
@@ -328,6 +340,7 @@ void adamw_step(handle params_, handle grads, handle exp_avgs, handle exp_avg_sq
   const char *what = "adamw_step";
   const Tensors ps(params_, what), gs(grads, what), ms(exp_avgs, what), vs(exp_avg_sqs, what);
   const lpg_adamw_hyper h = hyper(what, step, lr, betas, eps, weight_decay);
+  no_tangent(what, grad_scale);
   if (ps.empty()) return;
   const int32_t type = params(what, ps);
   same(what, "grads", gs, ps, ps[0].scalar_type());
@@ -365,6 +378,7 @@ void adamw_step_8bit(handle params_, handle grads, handle m8_, handle m_scales, 
   const char *what = "adamw_step_8bit";
   const Tensors ps(params_, what), gs(grads, what), m8(m8_, what), ms(m_scales, what), r8(r8_, what), rs(r_scales, what);
   const lpg_adamw_hyper h = hyper(what, step, lr, betas, eps, weight_decay);
+  no_tangent(what, grad_scale);
   if (ps.empty()) return;
   const int32_t type = params(what, ps);
   REQUIRE(!places || places->size() == ps.size(), "lpgnn ", what, ": ", ps.size(), " params and ", places->size(),
@@ -407,6 +421,8 @@ std::pair<Tensor, Tensor> clip_scale(handle grads, double max_norm) {
 // ------------------------------------------------------------------ 8-bit integers
 // x [.., K1] (and x2 [.., K2], the same rows) as row matrices
 std::pair<Tensor, Tensor> i8_rows(const char *what, const Tensor &x, const OptTensor &x2) {
+  no_tangent(what, x);
+  no_tangent(what, x2);
   REQUIRE(x.is_cuda(), "lpgnn ", what, ": runs on a HIP device only (no CPU path)");
   REQUIRE(code_of(x.scalar_type()) >= 0, "lpgnn ", what, ": x must be float32, bfloat16 or float16, got ",
           x.scalar_type());
@@ -446,6 +462,8 @@ std::pair<Tensor, Tensor> quantize_i8(const Tensor &x, const OptTensor &x2) {
 Tensor linear_i8(const Tensor &x, const Tensor &wq, const Tensor &ws, const OptTensor &bias, const OptTensor &x2,
                  bool relu) {
   const char *what = "linear_i8";
+  no_tangent(what, ws);
+  no_tangent(what, bias);
   const auto [a, b] = i8_rows(what, x, x2);
   const int64_t M = a.size(0), K1 = a.size(1), K2 = b.defined() ? b.size(1) : 0, K = K1 + K2;
   REQUIRE(wq.dim() == 2 && wq.scalar_type() == at::kChar && wq.device() == x.device() && wq.size(1) == K && wq.size(0) > 0,

@@ -7,8 +7,8 @@ torch.nn.LayerNorm names them); ``GCN_FC(..., norm="layer")`` puts one behind ev
 side.  x fp32, bf16 or fp16 with any row stride; weight and bias fp32 (the master weights of bf16
 training) or x's own type; statistics and sums in fp32, the output rounded once to x's type.  The
 backward returns dx in x's type and the weight gradients in theirs, from a deterministic reduction.
-There is no CPU path and no second derivative (a backward through gradients raises).  The argument
-checks and the autograd node are C++ (csrc/host.cpp).
+There is no CPU path, no forward-mode derivative (a tensor with a tangent raises) and no second derivative
+(a backward through gradients raises).  The argument checks and the autograd node are C++ (csrc/host.cpp).
 """
 from __future__ import annotations
 

@@ -9,8 +9,8 @@ features) and W = [W_rel | W_root]:
     y_mn  = act((sum_k q_mk wq_nk) (top_m / 127) ws_n + bias_n)
 
 The sum is exact (32-bit integers), the quotient decided exactly, so the result does not depend on how the
-work is split.  x fp32, bf16 or fp16, y of its type.  No gradient; no CPU path.  Checks and launches are
-C++ (csrc/host.cpp).
+work is split.  x fp32, bf16 or fp16, y of its type.  No gradient, backward or forward-mode
+(both refused); no CPU path.  Checks and launches are C++ (csrc/host.cpp).
 """
 from __future__ import annotations
 

@@ -68,3 +68,18 @@ def test_reference_gradients_against_differences(relu):
         hi[k], lo[k] = t + 1e-5 * d, t - 1e-5 * d
         diff = (f(*hi) - f(*lo)) / 2e-5
         assert abs(diff - (got[k] * d).sum()) < 1e-7
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "bias"])
+def test_refuses_forward_mode_tangents(which):
+    """A dual tensor would come out without its tangent, which reads as a derivative of zero."""
+    import torch.autograd.forward_ad as fwd
+
+    from lpgnn import layer_norm
+
+    ts = dict(x=torch.ones(2, 4), weight=torch.ones(4), bias=torch.ones(4))
+    with fwd.dual_level():
+        ts[which] = fwd.make_dual(ts[which], torch.ones_like(ts[which]))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                layer_norm(**ts)

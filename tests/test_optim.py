@@ -105,3 +105,28 @@ def test_state_dict_round_trip_keeps_types():
     st = q.state[q.param_groups[0]["params"][0]]
     assert st["step"] == 7 and st["m8"].dtype == torch.float8_e4m3fn and st["r_scale"].dtype == torch.float32
     assert torch.equal(st["m_scale"], o.state[p]["m_scale"]) and st["m_scale"].data_ptr() != o.state[p]["m_scale"].data_ptr()
+
+
+def test_refuses_forward_mode_tangents():
+    """The updates drop a tangent, as a derivative of zero."""
+    import torch.autograd.forward_ad as fwd
+
+    from lpgnn import optim
+
+    t = lambda: torch.ones(3)
+    with fwd.dual_level(), torch.no_grad():
+        dual = fwd.make_dual(t(), t())
+        for k in range(4):
+            ts = [[t()] for _ in range(4)]
+            ts[k] = [dual]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                optim.adamw_step(*ts, step=1)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            optim.adamw_step([t()], [t()], [t()], [t()], step=1, grad_scale=dual)
+        for k in (0, 1, 3, 5):
+            ts = [[t()] for _ in range(6)]
+            ts[k] = [dual]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                optim.adamw_step_8bit(*ts, step=1)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            optim.clip_scale([dual], 1.0)

@@ -59,3 +59,20 @@ def test_chunk_rows():
     for M, N, K in ((10 ** 5, 1024, 2048), (10 ** 6, 100, 100), (10 ** 6, 2048, 4096), (10 ** 6, 10 ** 6, 131072)):
         rows = f(M, N, K)
         assert 0 < rows <= M and (rows == M or rows % 256 == 0)
+
+
+@pytest.mark.parametrize("which", ["x", "x2", "ws", "bias"])
+def test_refuses_forward_mode_tangents(which):
+    """A dual tensor would come out without its tangent, which reads as a derivative of zero."""
+    import torch.autograd.forward_ad as fwd
+
+    from lpgnn import linear_i8, quantize_i8
+
+    ts = dict(x=torch.ones(2, 16), x2=torch.ones(2, 16), ws=torch.ones(4), bias=torch.ones(4))
+    with fwd.dual_level(), torch.no_grad():
+        ts[which] = fwd.make_dual(ts[which], torch.ones_like(ts[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            linear_i8(wq=torch.ones(4, 32, dtype=torch.int8), **ts)
+        if which in ("x", "x2"):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                quantize_i8(ts["x"], ts["x2"])
