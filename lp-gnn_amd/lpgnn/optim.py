@@ -58,9 +58,10 @@ def clip_scale(grads, max_norm: float) -> tuple[Tensor, Tensor]:
 
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update on the kernels above.  ``state_bits``: 32 (state names and types as torch's,
-    whose state dicts it loads) or 8; ``max_grad_norm``: clip the gradients' global 2-norm inside the step (the
-    stored gradients are not changed; ``last_norm`` is the norm before the clip, a device scalar), over all
-    parameters of the optimizer, which then must share a type and a device; ``seed``: of the 8-bit rounding.
+    whose state dicts it loads, but for ``maximize`` and ``amsgrad``, which are refused) or 8;
+    ``max_grad_norm``: clip the gradients' global 2-norm inside the step (the stored gradients are not
+    changed; ``last_norm`` is the norm before the clip, a device scalar), over all parameters of the
+    optimizer, which then must share a type and a device; ``seed``: of the 8-bit rounding.
 
     Parameters float32 or bfloat16, contiguous, on HIP devices, gradients dense.  The step number is a host
     number, so ``step()`` refuses to be captured into a graph."""
@@ -76,6 +77,18 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.max_grad_norm, self.seed = int(state_bits), max_grad_norm, int(seed)
         self.last_norm = None
 
+    @staticmethod
+    def _refuse_others(groups) -> None:
+        """torch's options that make another update of it, which groups and state dicts may carry."""
+        for g in groups:
+            for k in ("maximize", "amsgrad"):
+                if g.get(k):
+                    raise RuntimeError(f"lpgnn AdamW: {k} is not supported")
+
+    def add_param_group(self, param_group) -> None:
+        self._refuse_others([param_group])
+        super().add_param_group(param_group)
+
     def _init(self, p: Tensor) -> dict:
         zeros = lambda n, dt: torch.zeros(n, dtype=dt, device=p.device)
         if self.state_bits == 32:
@@ -88,6 +101,7 @@ class AdamW(torch.optim.Optimizer):
     def step(self, closure=None):
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("lpgnn AdamW: step() cannot be captured into a graph (its step number would not advance)")
+        self._refuse_others(self.param_groups)
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -129,6 +143,7 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As torch's, but the moments keep their own types (torch would cast them to the parameter's)."""
+        self._refuse_others(state_dict["param_groups"])
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):

@@ -130,3 +130,28 @@ def test_refuses_forward_mode_tangents():
                 optim.adamw_step_8bit(*ts, step=1)
         with pytest.raises(RuntimeError, match="forward-mode"):
             optim.clip_scale([dual], 1.0)
+
+
+@pytest.mark.parametrize("flag", ["maximize", "amsgrad"])
+def test_refuses_other_updates_of_a_loaded_state(flag):
+    """torch's options that change the update: from a state dict, from a group, and set later."""
+    from lpgnn import optim
+
+    p = torch.nn.Parameter(torch.ones(3))
+    t = torch.optim.AdamW([p], **{flag: True})
+    p.grad = torch.ones(3)
+    t.step()
+    o = optim.AdamW([p])
+    with pytest.raises(RuntimeError, match=flag):
+        o.load_state_dict(t.state_dict())
+    assert not o.state and flag not in o.param_groups[0]  # nothing of it was taken
+    with pytest.raises(RuntimeError, match=flag):
+        optim.AdamW([{"params": [p], flag: True}])
+    with pytest.raises(RuntimeError, match=flag):
+        optim.AdamW([p]).add_param_group({"params": [torch.nn.Parameter(torch.ones(2))], flag: True})
+    o.param_groups[0][flag] = True
+    with pytest.raises(RuntimeError, match=flag):
+        o.step()
+    plain = torch.optim.AdamW([p], **{flag: False})
+    plain.step()
+    optim.AdamW([p]).load_state_dict(plain.state_dict())
