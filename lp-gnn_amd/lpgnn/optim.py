@@ -142,7 +142,8 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict) -> None:
-        """As torch's, but the moments keep their own types (torch would cast them to the parameter's)."""
+        """As torch's, but the moments keep their own types (torch would cast them to the parameter's): the 8-bit
+        codes, and fp32 for everything else, whatever the saved optimizer kept it in."""
         self._refuse_others(state_dict["param_groups"])
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
@@ -151,4 +152,5 @@ class AdamW(torch.optim.Optimizer):
                 if k == "step":
                     self.state[p][k] = int(v)
                 elif isinstance(v, Tensor):
-                    self.state[p][k] = v.to(device=p.device, copy=True).contiguous()
+                    dt = v.dtype if v.dtype == _F8 else torch.float32
+                    self.state[p][k] = v.to(device=p.device, dtype=dt, copy=True).contiguous()

@@ -477,3 +477,23 @@ def test_the_split_over_blocks_does_not_show(dtype):
     for x in (whole, cut):
         assert abs(x.double() - want) <= (2.0**-24 + n * 2.0**-53) * want
     assert abs(scale - scale2) <= 2.0**-22 * scale
+
+
+def test_goes_on_from_a_bf16_state_of_torch():
+    """torch keeps bf16 parameters' moments in bf16; the next step here is the kernel's from those numbers."""
+    from lpgnn import optim
+
+    ps = _model(2, torch.bfloat16)
+    t = torch.optim.AdamW(ps, **H)
+    for p in ps:
+        p.grad = torch.randn_like(p)
+    t.step()
+    a = optim.AdamW(ps, **H)
+    a.load_state_dict(t.state_dict())
+    host = [(p.detach().cpu(), p.grad.cpu(), t.state[p]["exp_avg"].float().cpu(), t.state[p]["exp_avg_sq"].float().cpu())
+            for p in ps]
+    a.step()
+    for p, x in zip(ps, host):
+        want = R.step32(*x, 2, **H)
+        for got, w in zip((p.detach(), a.state[p]["exp_avg"], a.state[p]["exp_avg_sq"]), want):
+            assert torch.equal(got.cpu(), w.to(got.dtype))

@@ -155,3 +155,21 @@ def test_refuses_other_updates_of_a_loaded_state(flag):
     plain = torch.optim.AdamW([p], **{flag: False})
     plain.step()
     optim.AdamW([p]).load_state_dict(plain.state_dict())
+
+
+def test_loads_moments_of_other_types():
+    """torch keeps the moments of bf16 parameters in bf16 (of fp64 ones in fp64): they become the fp32 the step takes."""
+    from lpgnn import optim
+
+    for dtype in (torch.bfloat16, torch.float64):
+        p = torch.nn.Parameter(torch.ones(5, dtype=dtype))
+        p.grad = torch.linspace(-1, 1, 5).to(dtype)
+        t = torch.optim.AdamW([p])
+        t.step()
+        q = torch.nn.Parameter(torch.ones(5, dtype=torch.bfloat16))
+        o = optim.AdamW([q])
+        o.load_state_dict(t.state_dict())
+        assert o.state[q]["step"] == 1
+        for k in ("exp_avg", "exp_avg_sq"):
+            assert t.state[p][k].dtype == dtype and o.state[q][k].dtype == torch.float32
+            assert torch.equal(o.state[q][k], t.state[p][k].float())
