@@ -77,6 +77,10 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.max_grad_norm, self.seed = int(state_bits), max_grad_norm, int(seed)
         self.last_norm = None
 
+    def __getstate__(self) -> dict:  # (torch's holds the groups and the state; __setstate__ takes whatever is in it)
+        own = {k: getattr(self, k) for k in ("state_bits", "max_grad_norm", "seed", "last_norm")}
+        return {**super().__getstate__(), **own}
+
     @staticmethod
     def _refuse_others(groups) -> None:
         """torch's options that make another update of it, which groups and state dicts may carry."""

@@ -497,3 +497,24 @@ def test_goes_on_from_a_bf16_state_of_torch():
         want = R.step32(*x, 2, **H)
         for got, w in zip((p.detach(), a.state[p]["exp_avg"], a.state[p]["exp_avg_sq"]), want):
             assert torch.equal(got.cpu(), w.to(got.dtype))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_deep_copy_steps_to_the_same_bits(bits):
+    import copy
+
+    from lpgnn import optim
+
+    ps = _model(3)
+    o = optim.AdamW(ps, state_bits=bits, max_grad_norm=0.7, seed=11)
+    for p in ps:
+        p.grad = torch.randn_like(p)
+    o.step()
+    c = copy.deepcopy(o)
+    qs = c.param_groups[0]["params"]
+    for p, q in zip(ps, qs):
+        p.grad = torch.randn_like(p)
+        q.grad = p.grad.clone()
+    o.step(), c.step()
+    assert all(torch.equal(p, q) and p.data_ptr() != q.data_ptr() for p, q in zip(ps, qs))
+    assert torch.equal(o.last_norm, c.last_norm)

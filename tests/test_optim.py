@@ -173,3 +173,23 @@ def test_loads_moments_of_other_types():
         for k in ("exp_avg", "exp_avg_sq"):
             assert t.state[p][k].dtype == dtype and o.state[q][k].dtype == torch.float32
             assert torch.equal(o.state[q][k], t.state[p][k].float())
+
+
+def test_copies_and_pickles_keep_the_settings():
+    """torch's Optimizer pickles and deep-copies its groups and state only."""
+    import copy
+    import io
+
+    from lpgnn import optim
+
+    p = torch.nn.Parameter(torch.ones(300))
+    o = optim.AdamW([p], state_bits=8, max_grad_norm=0.5, seed=7)
+    o.state[p].update(o._init(p))
+    o.last_norm = torch.tensor(3.0)
+    buf = io.BytesIO()
+    torch.save(o, buf)
+    buf.seek(0)
+    for c in (copy.deepcopy(o), torch.load(buf, weights_only=False)):
+        assert (c.state_bits, c.max_grad_norm, c.seed, c.last_norm) == (8, 0.5, 7, 3.0)
+        assert c.param_groups[0]["params"][0] is not p and len(c.state) == 1
+        assert c.state_dict().keys() == o.state_dict().keys()
