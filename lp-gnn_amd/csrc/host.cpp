@@ -419,16 +419,21 @@ std::pair<Tensor, Tensor> clip_scale(handle grads, double max_norm) {
 }
 
 // ------------------------------------------------------------------ 8-bit integers
+// whole numbers have no derivative: nothing a call computes from may want one
+void no_gradient(const char *what, const OptTensor &t) {
+  no_tangent(what, t);
+  REQUIRE(!at::GradMode::is_enabled() || !t || !t->requires_grad(), "lpgnn ", what,
+          ": 8-bit integers have no gradient (call it under torch.no_grad())");
+}
+
 // x [.., K1] (and x2 [.., K2], the same rows) as row matrices
 std::pair<Tensor, Tensor> i8_rows(const char *what, const Tensor &x, const OptTensor &x2) {
-  no_tangent(what, x);
-  no_tangent(what, x2);
+  no_gradient(what, x);
+  no_gradient(what, x2);
   REQUIRE(x.is_cuda(), "lpgnn ", what, ": runs on a HIP device only (no CPU path)");
   REQUIRE(code_of(x.scalar_type()) >= 0, "lpgnn ", what, ": x must be float32, bfloat16 or float16, got ",
           x.scalar_type());
   REQUIRE(x.dim() > 0 && x.size(-1) > 0, "lpgnn ", what, ": x needs columns, got shape ", x.sizes());
-  REQUIRE(!at::GradMode::is_enabled() || !(x.requires_grad() || (x2 && x2->requires_grad())), "lpgnn ", what,
-          ": 8-bit integers have no gradient (call it under torch.no_grad())");
   if (!x2) return {rows(x), Tensor()};
   REQUIRE(x2->device() == x.device() && x2->scalar_type() == x.scalar_type() && x2->dim() == x.dim() &&
               x2->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1) && x2->size(-1) > 0,
@@ -462,8 +467,8 @@ std::pair<Tensor, Tensor> quantize_i8(const Tensor &x, const OptTensor &x2) {
 Tensor linear_i8(const Tensor &x, const Tensor &wq, const Tensor &ws, const OptTensor &bias, const OptTensor &x2,
                  bool relu) {
   const char *what = "linear_i8";
-  no_tangent(what, ws);
-  no_tangent(what, bias);
+  no_gradient(what, ws);
+  no_gradient(what, bias);
   const auto [a, b] = i8_rows(what, x, x2);
   const int64_t M = a.size(0), K1 = a.size(1), K2 = b.defined() ? b.size(1) : 0, K = K1 + K2;
   REQUIRE(wq.dim() == 2 && wq.scalar_type() == at::kChar && wq.device() == x.device() && wq.size(1) == K && wq.size(0) > 0,

@@ -499,6 +499,7 @@ def two_direction_i8(left: Tensor, right: Tensor, adj: BipartiteCSR, layer, relu
                 raise RuntimeError("GCN_FC: the weights changed since quantize_int8(); call it again")
         return linear_i8(_spmm_forward(S, x_src, heavy=opts.spmm_heavy), wq, ws, bias, x2=x_dst, relu=relu)
 
-    if torch.is_grad_enabled() and (left.requires_grad or right.requires_grad):
+    params = (p for q in layer for p in q[4].parameters())
+    if torch.is_grad_enabled() and (left.requires_grad or right.requires_grad or any(p.requires_grad for p in params)):
         raise RuntimeError("GCN_FC: 8-bit evaluation has no gradient (call the model under torch.no_grad())")
     return direction(adj.fwd, right, left, layer[1]), direction(adj.bwd, left, right, layer[0])

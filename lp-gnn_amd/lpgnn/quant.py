@@ -10,7 +10,7 @@ features) and W = [W_rel | W_root]:
 
 The sum is exact (32-bit integers), the quotient decided exactly, so the result does not depend on how the
 work is split.  x fp32, bf16 or fp16, y of its type.  No gradient, backward or forward-mode
-(both refused); no CPU path.  Checks and launches are C++ (csrc/host.cpp).
+(refused where any tensor of the call wants one); no CPU path.  Checks and launches are C++ (csrc/host.cpp).
 """
 from __future__ import annotations
 

@@ -209,3 +209,18 @@ def test_command_line_trains_and_evaluates(tmp_path):
             ds = run.LPDataset(a.dataset_processed_prefix, thresh_num=a.edge_num_thresh, device=a.dev)
             _, acc, rows = run.validation(model, ds, a)
             assert 0 <= acc <= 1 and len(rows) == len(ds) and json.dumps(rows)
+
+
+def test_int8_refuses_gradients_of_hidden_layers_behind_frozen_ones():
+    """conv1 frozen, the hidden layers not: a loss would leave them without a gradient.  Frozen too, the heads train."""
+    from lpgnn import GCN_FC
+
+    batch, _ = _batch()
+    model = GCN_FC(8, 8, hids=32, depth=3).to(DEV).eval()
+    model.conv1.requires_grad_(False)
+    model.quantize_int8()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        model(batch)
+    model.layers.requires_grad_(False)
+    model(batch)[0].square().sum().backward()
+    assert model.lin_left.weight.grad is not None and model.conv1.left2right.lin_rel.weight.grad is None

@@ -49,3 +49,18 @@ def test_cli_flags():
     assert a.opt == "adamw8" and a.max_grad_norm == 0.5 and a.int8 == 1
     b = run.parse_args([])
     assert b.max_grad_norm == 0 and b.int8 == 0
+
+
+@pytest.mark.parametrize("name", ["lin_rel.weight", "lin_rel.bias", "lin_root.weight"])
+def test_int8_layer_refuses_weights_that_want_a_gradient(name):
+    """Also where its inputs want none (the layers before it frozen): the weights would silently get no gradient."""
+    from lpgnn.arch import GraphConvTwoDirection
+    from lpgnn.conv import two_direction_i8
+
+    layer = GraphConvTwoDirection(4, 4, 4)
+    for side in ("left2right", "right2left"):
+        layer.requires_grad_(False)
+        layer.get_parameter(f"{side}.{name}").requires_grad_(True)
+        codes = [(None, None, None, [], d) for d in (layer.left2right, layer.right2left)]
+        with pytest.raises(RuntimeError, match="no gradient"):
+            two_direction_i8(torch.ones(2, 4), torch.ones(3, 4), None, codes, True)

@@ -76,3 +76,16 @@ def test_refuses_forward_mode_tangents(which):
         if which in ("x", "x2"):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 quantize_i8(ts["x"], ts["x2"])
+
+
+@pytest.mark.parametrize("which", ["x", "x2", "ws", "bias"])
+def test_refuses_whatever_wants_a_gradient(which):
+    from lpgnn import linear_i8
+
+    ts = dict(x=torch.ones(2, 16), x2=torch.ones(2, 16), ws=torch.ones(4), bias=torch.ones(4))
+    ts[which].requires_grad_(True)
+    wq = torch.ones(4, 32, dtype=torch.int8)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        linear_i8(wq=wq, **ts)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):  # (what a host tensor is refused for)
+        linear_i8(wq=wq, **ts)
