@@ -72,6 +72,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"lpgnn AdamW: state_bits must be 8 or 32, got {state_bits}")
         if max_grad_norm is not None and not max_grad_norm >= 0:
             raise ValueError(f"lpgnn AdamW: max_grad_norm must not be negative, got {max_grad_norm}")
+        if not 0 <= int(seed) < 1 << 64:
+            raise ValueError(f"lpgnn AdamW: seed must be a whole number of 64 bits, got {seed}")
         adamw_step([], [], [], [], step=1, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)  # (checks them)
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
         self.state_bits, self.max_grad_norm, self.seed = int(state_bits), max_grad_norm, int(seed)

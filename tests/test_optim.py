@@ -193,3 +193,14 @@ def test_copies_and_pickles_keep_the_settings():
         assert (c.state_bits, c.max_grad_norm, c.seed, c.last_norm) == (8, 0.5, 7, 3.0)
         assert c.param_groups[0]["params"][0] is not p and len(c.state) == 1
         assert c.state_dict().keys() == o.state_dict().keys()
+
+
+def test_seed_is_checked_where_it_is_given():
+    """The 8-bit rounding's seed is 64 bits: refused where it is given, not in the first step."""
+    from lpgnn import optim
+
+    p = torch.nn.Parameter(torch.ones(3))
+    for seed in (-1, 1 << 64):
+        with pytest.raises(ValueError, match="seed"):
+            optim.AdamW([p], state_bits=8, seed=seed)
+    assert optim.AdamW([p], state_bits=8, seed=(1 << 64) - 1).seed == (1 << 64) - 1
