@@ -283,12 +283,12 @@ struct Spans {
     bool out;
   };
   std::vector<Span> list;
+  void add(const Tensor &t, bool out) {
+    const char *p = static_cast<const char *>(t.data_ptr());
+    if (t.numel() > 0) list.push_back({p, p + t.numel() * t.element_size(), out});
+  }
   void add(const Tensors &ts, bool out) {
-    for (size_t i = 0; i < ts.size(); ++i) {
-      const Tensor &t = ts[i];
-      const char *p = static_cast<const char *>(t.data_ptr());
-      if (t.numel() > 0) list.push_back({p, p + t.numel() * t.element_size(), out});
-    }
+    for (size_t i = 0; i < ts.size(); ++i) add(ts[i], out);
   }
   void check(const char *what) {
     std::sort(list.begin(), list.end(), [](const Span &a, const Span &b) { return a.at < b.at; });
@@ -301,10 +301,11 @@ struct Spans {
     }
   }
 };
-void apart(const char *what, const Tensors &gs, std::initializer_list<const Tensors *> written) {
+void apart(const char *what, const Tensors &gs, const OptTensor &scale, std::initializer_list<const Tensors *> written) {
   Spans s;
-  s.list.reserve(gs.size() * (1 + written.size()));
+  s.list.reserve(gs.size() * (1 + written.size()) + 1);
   s.add(gs, false);
+  if (scale) s.add(*scale, false);
   for (const Tensors *ts : written) s.add(*ts, true);
   s.check(what);
 }
@@ -347,7 +348,7 @@ void adamw_step(handle params_, handle grads, handle exp_avgs, handle exp_avg_sq
   same(what, "exp_avgs", ms, ps, at::kFloat);
   same(what, "exp_avg_sqs", vs, ps, at::kFloat);
   const float *scale = scale_ptr(what, grad_scale, ps);
-  apart(what, gs, {&ps, &ms, &vs});
+  apart(what, gs, grad_scale, {&ps, &ms, &vs});
   std::vector<lpg_adamw_tensor> tab(ps.size());
   for (size_t i = 0; i < ps.size(); ++i)
     tab[i] = {ps[i].data_ptr(), gs[i].data_ptr(), ptr_of<float>(ms[i]), ptr_of<float>(vs[i]), ps[i].numel()};
@@ -389,7 +390,7 @@ void adamw_step_8bit(handle params_, handle grads, handle m8_, handle m_scales, 
   same(what, "r8", r8, ps, at::kFloat8_e4m3fn);
   same(what, "r_scales", rs, ps, at::kFloat, true);
   const float *scale = scale_ptr(what, grad_scale, ps);
-  apart(what, gs, {&ps, &m8, &ms, &r8, &rs});
+  apart(what, gs, grad_scale, {&ps, &m8, &ms, &r8, &rs});
   std::vector<lpg_adamw8_tensor> tab(ps.size());
   for (size_t i = 0; i < ps.size(); ++i)
     tab[i] = {ps[i].data_ptr(), gs[i].data_ptr(),      m8[i].data_ptr(), ptr_of<float>(ms[i]),

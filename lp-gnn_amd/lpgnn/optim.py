@@ -34,7 +34,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 1
     """One AdamW step (number ``step``, from 1) over lists of contiguous tensors, in place.  params and grads
     float32 or bfloat16 (one type a call), the moments float32; the update is computed in fp32 and rounded
     once.  ``grad_scale``: a device scalar every gradient is multiplied by (``clip_scale``).  No tensor
-    that is written may overlap another of the call (refused); gradients may share memory."""
+    that is written may overlap another of the call, ``grad_scale`` among them (refused); gradients may share
+    memory."""
     _lib.host().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, grad_scale)
 
 

@@ -518,3 +518,20 @@ def test_a_deep_copy_steps_to_the_same_bits(bits):
     o.step(), c.step()
     assert all(torch.equal(p, q) and p.data_ptr() != q.data_ptr() for p, q in zip(ps, qs))
     assert torch.equal(o.last_norm, c.last_norm)
+
+
+def test_a_scale_inside_a_written_tensor_is_refused():
+    """grad_scale is read by every block while others write: it may share memory with a gradient only."""
+    from lpgnn import optim
+
+    t = lambda: torch.zeros(300, device=DEV)
+    p, g, m, v = t(), t(), t(), t()
+    for s in (p[:1], p[299:], m[5], v[7:8]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            optim.adamw_step([p], [g], [m], [v], step=1, grad_scale=s)
+    optim.adamw_step([p], [g], [m], [v], step=1, grad_scale=g[3])
+    q = [torch.zeros(300, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for _ in range(2)]
+    s = [torch.zeros(2, device=DEV) for _ in range(2)]
+    for scale in (p[1:2], s[0][0], s[1][1]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            optim.adamw_step_8bit([p], [g], [q[0]], [s[0]], [q[1]], [s[1]], step=1, grad_scale=scale)
