@@ -185,7 +185,7 @@ class GCN_FC(GCNBase):
         self.dp = dp
         if norm == "layer":
             self.norms = nn.ModuleList(nn.ModuleDict(dict(left=LayerNorm(hids), right=LayerNorm(hids)))
-                                       for _ in range(depth - 1))
+                                       for _ in range(1 + len(self.layers)))
         else:
             self.norms = None
         self._int8 = None

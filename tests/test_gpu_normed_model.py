@@ -224,3 +224,15 @@ def test_int8_refuses_gradients_of_hidden_layers_behind_frozen_ones():
     model.layers.requires_grad_(False)
     model(batch)[0].square().sum().backward()
     assert model.lin_left.weight.grad is not None and model.conv1.left2right.lin_rel.weight.grad is None
+
+
+def test_the_shallowest_model():
+    """depth=1 is conv1 and the heads, as depth=2."""
+    from lpgnn import GCN_FC
+
+    batch, A = _batch()
+    torch.manual_seed(4)
+    model = GCN_FC(8, 8, hids=32, depth=1, norm="layer").to(DEV)
+    lc, lv = model(batch)
+    (rc, rv), _ = _model64(model, batch, A)  # (bound: test_forward_and_gradients)
+    assert (lc.cpu().double() - rc).abs().max() < 1e-3 and (lv.cpu().double() - rv).abs().max() < 1e-3

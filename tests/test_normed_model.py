@@ -64,3 +64,12 @@ def test_int8_layer_refuses_weights_that_want_a_gradient(name):
         codes = [(None, None, None, [], d) for d in (layer.left2right, layer.right2left)]
         with pytest.raises(RuntimeError, match="no gradient"):
             two_direction_i8(torch.ones(2, 4), torch.ones(3, 4), None, codes, True)
+
+
+@pytest.mark.parametrize("depth", [0, 1, 2, 5])
+def test_a_norm_behind_every_layer(depth):
+    """conv1 is there whatever the depth (arch.py:170-174), and so is its norm."""
+    from lpgnn import GCN_FC
+
+    m = GCN_FC(8, 8, hids=16, depth=depth, norm="layer")
+    assert len(m.norms) == 1 + len(m.layers) == max(depth - 1, 1)
