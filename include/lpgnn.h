@@ -775,7 +775,8 @@ lpg_status lpg_layer_norm_bwd(int32_t dtype, int32_t wdtype, int64_t M, int64_t 
  * each product and sum rounded to fp32.  At step t: rest = 1 - beta, inv_root2 = 1 / sqrt(1 - beta2^t),
  * keep = 1 - lr weight_decay, rate = lr / (1 - beta1^t).  p and g contiguous, of `dtype` (LPG_F32 or
  * LPG_BF16), any element alignment; m / v fp32.  No two tensors of a call may overlap.  `tensors` is a
- * host array, read during the call; n = 0 is skipped.
+ * host array, read during the call; n = 0 is skipped; a tensor of 2^36 numbers or more (2^34 with 8-bit
+ * moments), past what a launch holds, is LPG_ERR_UNSUPPORTED.
  * lpg_adamw8: the moments in 8 bits.  m8 / r8: n e4m3 numbers (OCP), ms / rs: ceil(n / 256) fp32 scales;
  * m = m8 ms, sqrt(v) = r8 rs of the element's block of 256.  Rounding adds 16 bits of a hash of
  * key ^ element below the kept mantissa (key: one per tensor and step).  All zeros = no history yet. */

@@ -389,7 +389,7 @@ lpg_status in_tables(Tab &tab, int many, int64_t chunk, int64_t count, const E *
     for (; at < count && k < many; ++at) {
       if (list[at].n == 0) continue;
       const int64_t b = blocks_of(list[at].n, chunk);
-      if (blocks + b > INT32_MAX) {
+      if (blocks + b > most_blocks(kT)) {
         if (k == 0) {
           set_error("%s: a tensor of %lld elements is too large", what, (long long)list[at].n);
           return LPG_ERR_UNSUPPORTED;

@@ -34,6 +34,9 @@ inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s);
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Blocks of `threads` that a launch holds in a dimension: fewer than 2^32 threads.
+constexpr int64_t most_blocks(int threads) { return (int64_t)UINT32_MAX / threads; }
+
 // Compute units of the current device (cached per device id).
 inline int device_cus() {
   static int cus[64] = {0};

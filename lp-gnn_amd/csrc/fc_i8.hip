@@ -811,7 +811,7 @@ lpg_status run_rows(const RowsArgs &a, hipStream_t s) {
 // 10.6), and with more blocks the rows that each quantises again cost more than the launch (2000 x 512, K = 256 13.6
 // and 7.3).
 bool few_rows(int64_t M, int64_t N, int64_t K) {
-  if (M <= 1) return (K + 1023) / 1024 * 1024 <= kRowBytes;
+  if (M <= 1) return (K + 1023) / 1024 * 1024 <= kRowBytes && (N + 3) / 4 <= most_blocks(256);
   return K <= kSomeK && (M + 15) / 16 <= 65535 && (M + 15) / 16 * ((N + kSomeN - 1) / kSomeN) <= device_cus();
 }
 
@@ -852,15 +852,22 @@ extern "C" lpg_status lpg_quant_i8(int32_t dtype, int64_t M, int64_t K1, const v
   LPG_REQUIRE(ldq >= K1 + K2 && ldq % 128 == 0, "lpg_quant_i8: ldq must be a multiple of 128 that holds K1 + K2");
   LPG_REQUIRE(M == 0 || (x && q && scale && (K2 == 0 || x2)), "lpg_quant_i8: NULL pointer");
   LPG_REQUIRE(aligned16(q), "lpg_quant_i8: q must be 16-byte aligned");
-  LPG_REQUIRE((M + 3) / 4 <= INT32_MAX, "lpg_quant_i8: too many rows");
   // x past the caches where it would push out the codes (100 K x 2048 fp32 with the product to 1024 469 -> 394 us, 60 K x
   // 2048 fp16 187 -> 177); a small x may still be in them (20000 x 1024 fp16 45 us through them, 47 past them)
   const int past = M * (K1 + K2) * (dtype == LPG_F32 ? 4 : 2) > (int64_t)128 << 20;
   const QuantArgs a{M, ldx, ldx2, ldq, (int)K1, (int)K2, x, x2, q, scale, past};
   const auto go = [&](auto kernel, int rows) -> lpg_status {
-    if (M == 0) return LPG_OK;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((M + rows - 1) / rows)), dim3(256), 0, as_stream(stream), a);
-    LPG_HIP(hipGetLastError());
+    const int64_t most = most_blocks(256) * rows, e = dtype == LPG_F32 ? 4 : 2;
+    for (int64_t at = 0; at < M; at += most) {  // (one launch but for tens of millions of rows)
+      QuantArgs b = a;
+      b.M = M - at < most ? M - at : most;
+      b.x = static_cast<const char *>(x) + at * ldx * e;
+      b.x2 = K2 ? static_cast<const char *>(x2) + at * ldx2 * e : nullptr;
+      b.q = q + at * ldq;
+      b.scale = scale + at;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)((b.M + rows - 1) / rows)), dim3(256), 0, as_stream(stream), b);
+      LPG_HIP(hipGetLastError());
+    }
     return LPG_OK;
   };
   // The fewest lanes, from 8 on, that hold a row in up to four vectors each, else a wave and up to 16 vectors a lane:

@@ -297,3 +297,20 @@ def test_one_tensor_as_both_parts():
     assert torch.equal(linear_i8(xd, wq, ws, _dev(bias), x2=xd), linear_i8(xd.repeat(1, 2), wq, ws, _dev(bias)))
     rows = xd[:1].expand(70, 24)  # a broadcast input
     assert torch.equal(linear_i8(rows, wq, ws, x2=rows), linear_i8(rows.contiguous(), wq, ws, x2=rows.contiguous()))
+
+
+def test_more_rows_than_a_launch_holds():
+    """Four rows a block of 256 threads, fewer than 2^32 threads a launch: rows past 2^26 have their codes too."""
+    from lpgnn import quantize_i8
+
+    M, K = 2**26 + 77, 72
+    x = torch.zeros(M, 1, dtype=torch.float16, device=DEV)
+    x2 = torch.zeros(M, K, dtype=torch.float16, device=DEV)
+    for t in (x, x2):
+        t[:100].normal_()
+        t[-200:].normal_()
+    q, s = quantize_i8(x, x2)
+    for a, b in ((0, 300), (M - 300, M)):
+        q0, s0 = quantize_i8(x[a:b].clone(), x2[a:b].clone())
+        assert torch.equal(q[a:b], q0) and torch.equal(s[a:b], s0)
+    assert s.count_nonzero() == 300

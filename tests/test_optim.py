@@ -204,3 +204,19 @@ def test_seed_is_checked_where_it_is_given():
         with pytest.raises(ValueError, match="seed"):
             optim.AdamW([p], state_bits=8, seed=seed)
     assert optim.AdamW([p], state_bits=8, seed=(1 << 64) - 1).seed == (1 << 64) - 1
+
+
+def test_c_entries_refuse_more_blocks_than_a_launch_holds():
+    """Fewer than 2^32 threads a launch: 2^24 blocks of 256 are too many (numbers a block: 4096, 1024, 16384)."""
+    import ctypes
+
+    from lpgnn import _lib
+
+    L = _lib.lib()
+    h = _lib.LpgAdamwHyper(0.9, 0.1, 0.999, 0.001, 1.0, 1e-8, 1.0, 1e-3)
+    p = 1 << 20  # never dereferenced
+    i64 = lambda *a: (ctypes.c_int64 * len(a))(*a)
+    assert L.lpg_adamw(2, 1, i64(p, p, p, p, 1 << 36), h, None, None) == 3 and b"too large" in L.lpg_last_error()
+    assert L.lpg_adamw8(2, 1, i64(p, p, p, p, p, p, 1 << 34, 0), h, None, None) == 3
+    assert b"too large" in L.lpg_last_error()
+    assert L.lpg_grad_norm(2, 1, i64(p, 1 << 38), 1.0, p, p, p, None) == 3 and b"too large" in L.lpg_last_error()

@@ -89,3 +89,11 @@ def test_refuses_whatever_wants_a_gradient(which):
         linear_i8(wq=wq, **ts)
     with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):  # (what a host tensor is refused for)
         linear_i8(wq=wq, **ts)
+
+
+def test_c_entry_of_one_row_refuses_more_blocks_than_a_launch_holds():
+    """Four columns a block of 256 threads, fewer than 2^32 threads a launch: the two launches take it."""
+    from lpgnn import _lib
+
+    p, N = 1 << 20, 1 << 26
+    assert _lib.lib().lpg_fc_i8_rows(2, 1, N, 16, p, 16, 0, None, 0, p, 16, p, None, 0, p, N, None) == 3
