@@ -14,6 +14,7 @@
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -23,6 +24,8 @@
 #include <initializer_list>
 #include <optional>
 #include <stdexcept>
+#include <unordered_set>
+#include <vector>
 
 #include "lpgnn.h"
 
@@ -188,6 +191,32 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 };
 
+// A backward that is captured while an eager graph of the same leaves lives would add to their gradients on the eager
+// graph's stream, out of the capture, which ends the process: refused in the forward, before there is one.  The leaves
+// are those behind t's whole graph (a view or a cast of a parameter has the parameter's).
+void no_eager_leaf(const Tensor &t) {
+  using torch::autograd::Node;
+  const auto id = c10::hip::getCurrentHIPStream(t.get_device()).id();
+  const auto check_leaf = [&](Node *acc) {
+    const auto stream = acc->stream();
+    REQUIRE(!stream || stream->id() == id,
+            "lpgnn layer_norm: captured while an eager autograd graph of the same parameters lives; drop it first");
+  };
+  if (t.is_leaf()) {
+    if (const auto acc = torch::autograd::impl::try_get_grad_accumulator(t)) check_leaf(acc.get());
+    return;
+  }
+  std::unordered_set<Node *> seen{t.grad_fn().get()};
+  std::vector<Node *> todo(seen.begin(), seen.end());
+  while (!todo.empty()) {
+    Node *const n = todo.back();
+    todo.pop_back();
+    if (dynamic_cast<torch::autograd::AccumulateGrad *>(n)) check_leaf(n);
+    for (const auto &e : n->next_edges())
+      if (e.function && seen.insert(e.function.get()).second) todo.push_back(e.function.get());
+  }
+}
+
 Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double eps, bool relu) {
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
   for (const Tensor *t : {&x, &w, &b}) no_tangent("layer_norm", *t);
@@ -207,18 +236,10 @@ Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bia
   REQUIRE(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
           "lpgnn layer_norm: weight and bias must share a type, got ", w.scalar_type(), " and ", b.scalar_type());
   const auto grad = [](const Tensor &t) { return t.defined() && t.requires_grad(); };
-  // A backward that is captured while an eager graph of the same leaves lives would add to their gradients on
-  // the eager graph's stream, out of the capture, which ends the process: refused here, before there is one.
   const c10::DeviceGuard guard(x.device());
-  if (at::GradMode::is_enabled() && capturing()) {
-    for (const Tensor &t : {x, w, b}) {
-      if (!grad(t) || !t.is_leaf()) continue;
-      const auto acc = torch::autograd::impl::try_get_grad_accumulator(t);
-      const auto stream = acc ? acc->stream() : std::nullopt;
-      REQUIRE(!stream || stream->id() == c10::hip::getCurrentHIPStream(t.get_device()).id(),
-              "lpgnn layer_norm: captured while an eager autograd graph of the same parameters lives; drop it first");
-    }
-  }
+  if (at::GradMode::is_enabled() && capturing())
+    for (const Tensor *t : {&x, &w, &b})
+      if (grad(*t)) no_eager_leaf(*t);
   const auto packed = [](const OptTensor &t) { return t ? OptTensor(t->contiguous()) : t; };
   const Tensor xr = rows(x);
   const OptTensor wc = packed(weight), bc = packed(bias);

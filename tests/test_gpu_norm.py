@@ -330,3 +330,35 @@ def test_gradients_of_shared_and_broadcast_inputs():
     r = x[:1].clone().requires_grad_(True)
     want, = torch.autograd.grad(layer_norm(r, w, None, EPS), r, dy[:1])
     assert y.shape == (D,) and torch.equal(g, want[0])
+
+
+def test_capture_beside_an_eager_graph_of_a_view_is_refused():
+    """The parameters of the call may be views or casts of the leaves that the eager graph holds; within one capture
+    they may be used as often as wanted."""
+    from lpgnn import layer_norm
+
+    x = torch.randn(8, 16, device=DEV)
+    both = torch.rand(2, 16, device=DEV).add_(0.5).requires_grad_(True)  # weight and bias its two rows
+
+    def norm(x):
+        return layer_norm(x, both[0], both[1].clone())
+
+    alive = norm(x).sum()
+    for make in (lambda: norm(x), lambda: layer_norm(x + both[0])):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager autograd graph"):
+            with torch.cuda.graph(graph):
+                make()
+        torch.cuda.synchronize()
+    del alive, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = norm(norm(x))
+        g, = torch.autograd.grad(y.sum(), both)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        e = norm(norm(x))
+        eg, = torch.autograd.grad(e.sum(), both)
+        assert torch.equal(y, e) and torch.equal(g, eg)
+        del e, eg
