@@ -358,7 +358,8 @@ void written(const Tensors &ts) {
 using pybind11::handle;
 
 void adamw_step(handle params_, handle grads, handle exp_avgs, handle exp_avg_sqs, int64_t step, double lr,
-                std::pair<double, double> betas, double eps, double weight_decay, const OptTensor &grad_scale) {
+                std::pair<double, double> betas, double eps, double weight_decay, const OptTensor &grad_scale,
+                bool check_only) {
   const char *what = "adamw_step";
   const Tensors ps(params_, what), gs(grads, what), ms(exp_avgs, what), vs(exp_avg_sqs, what);
   const lpg_adamw_hyper h = hyper(what, step, lr, betas, eps, weight_decay);
@@ -370,6 +371,7 @@ void adamw_step(handle params_, handle grads, handle exp_avgs, handle exp_avg_sq
   same(what, "exp_avg_sqs", vs, ps, at::kFloat);
   const float *scale = scale_ptr(what, grad_scale, ps);
   apart(what, gs, grad_scale, {&ps, &ms, &vs});
+  if (check_only) return;
   std::vector<lpg_adamw_tensor> tab(ps.size());
   for (size_t i = 0; i < ps.size(); ++i)
     tab[i] = {ps[i].data_ptr(), gs[i].data_ptr(), ptr_of<float>(ms[i]), ptr_of<float>(vs[i]), ps[i].numel()};
@@ -396,7 +398,8 @@ int64_t rounding_key(int64_t place, int64_t step, uint64_t seed) {
 
 void adamw_step_8bit(handle params_, handle grads, handle m8_, handle m_scales, handle r8_, handle r_scales,
                      const std::optional<std::vector<int64_t>> &places, uint64_t seed, int64_t step, double lr,
-                     std::pair<double, double> betas, double eps, double weight_decay, const OptTensor &grad_scale) {
+                     std::pair<double, double> betas, double eps, double weight_decay, const OptTensor &grad_scale,
+                     bool check_only) {
   const char *what = "adamw_step_8bit";
   const Tensors ps(params_, what), gs(grads, what), m8(m8_, what), ms(m_scales, what), r8(r8_, what), rs(r_scales, what);
   const lpg_adamw_hyper h = hyper(what, step, lr, betas, eps, weight_decay);
@@ -412,6 +415,7 @@ void adamw_step_8bit(handle params_, handle grads, handle m8_, handle m_scales, 
   same(what, "r_scales", rs, ps, at::kFloat, true);
   const float *scale = scale_ptr(what, grad_scale, ps);
   apart(what, gs, grad_scale, {&ps, &m8, &ms, &r8, &rs});
+  if (check_only) return;
   std::vector<lpg_adamw8_tensor> tab(ps.size());
   for (size_t i = 0; i < ps.size(); ++i)
     tab[i] = {ps[i].data_ptr(), gs[i].data_ptr(),      m8[i].data_ptr(), ptr_of<float>(ms[i]),

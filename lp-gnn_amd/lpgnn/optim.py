@@ -36,7 +36,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 1
     once.  ``grad_scale``: a device scalar every gradient is multiplied by (``clip_scale``).  No tensor
     that is written may overlap another of the call, ``grad_scale`` among them (refused); gradients may share
     memory."""
-    _lib.host().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, grad_scale)
+    _lib.host().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, grad_scale, False)
 
 
 def adamw_step_8bit(params, grads, m8, m_scales, r8, r_scales, *, step: int, seed: int = 0, lr: float = 1e-3,
@@ -46,7 +46,7 @@ def adamw_step_8bit(params, grads, m8, m_scales, r8, r_scales, *, step: int, see
     r_scales (float32, one a block of 256 elements), all zero before the first step.  ``places``: the tensors'
     places in the rounding's numbering (default 0, 1, ...), for a call on part of a model's list."""
     _lib.host().adamw_step_8bit(params, grads, m8, m_scales, r8, r_scales, places, seed, step, lr, betas, eps,
-                                weight_decay, grad_scale)
+                                weight_decay, grad_scale, False)
 
 
 def clip_scale(grads, max_norm: float) -> tuple[Tensor, Tensor]:
@@ -132,20 +132,28 @@ class AdamW(torch.optim.Optimizer):
                 # one launch per group, type, device and step number
                 calls.setdefault((gi, p.dtype, p.device, int(st["step"]) + 1), []).append((p, g, st, place - 1))
         scale = None
+
+        def update(key, items, check_only):
+            group, step = self.param_groups[key[0]], key[3]
+            ps, gs, sts, places = zip(*items)
+            of = lambda k: [s[k] for s in sts]
+            hyper = (step, float(group["lr"]), group["betas"], group["eps"], group["weight_decay"], scale, check_only)
+            if self.state_bits == 32:
+                _lib.host().adamw_step(ps, gs, of("exp_avg"), of("exp_avg_sq"), *hyper)
+            else:
+                _lib.host().adamw_step_8bit(ps, gs, of("m8"), of("m_scale"), of("r8"), of("r_scale"), places, self.seed,
+                                            *hyper)
+            if not check_only:
+                for s in sts:
+                    s["step"] = step
+
+        if len(calls) > 1:  # no parameter is updated where another's call is refused (one call checks all of its own)
+            for key, items in calls.items():
+                update(key, items, True)
         if self.max_grad_norm is not None and grads:
             self.last_norm, scale = clip_scale(grads, self.max_grad_norm)
-        for (gi, _, _, step), items in calls.items():
-            group = self.param_groups[gi]
-            ps, gs, sts, places = zip(*items)
-            kw = dict(step=step, lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
-                      weight_decay=group["weight_decay"], grad_scale=scale)
-            if self.state_bits == 32:
-                adamw_step(ps, gs, [s["exp_avg"] for s in sts], [s["exp_avg_sq"] for s in sts], **kw)
-            else:
-                adamw_step_8bit(ps, gs, [s["m8"] for s in sts], [s["m_scale"] for s in sts], [s["r8"] for s in sts],
-                                [s["r_scale"] for s in sts], seed=self.seed, places=places, **kw)
-            for p, s in zip(ps, sts):
-                s["step"] = step
+        for key, items in calls.items():
+            update(key, items, False)
         return loss
 
     def load_state_dict(self, state_dict) -> None:

@@ -535,3 +535,19 @@ def test_a_scale_inside_a_written_tensor_is_refused():
     for scale in (p[1:2], s[0][0], s[1][1]):
         with pytest.raises(RuntimeError, match="overlap"):
             optim.adamw_step_8bit([p], [g], [q[0]], [s[0]], [q[1]], [s[1]], step=1, grad_scale=scale)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_refused_step_updates_nothing(bits):
+    """Two groups, the second with a parameter that its call refuses: the first is as it was, and steps once after."""
+    from lpgnn import optim
+
+    a = torch.nn.Parameter(torch.ones(40, device=DEV))
+    b = torch.nn.Parameter(torch.ones(8, 6, device=DEV).t())
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    for most in (None, 1.0):
+        o = optim.AdamW([dict(params=[a]), dict(params=[b], lr=0.1)], state_bits=bits, max_grad_norm=most)
+        with pytest.raises(RuntimeError, match="contiguous"):
+            o.step()
+        assert torch.equal(a, torch.ones_like(a)) and o.state[a]["step"] == 0 and o.last_norm is None
+        assert not any(t.float().any() for t in o.state[a].values() if isinstance(t, torch.Tensor))
