@@ -362,3 +362,28 @@ def test_capture_beside_an_eager_graph_of_a_view_is_refused():
         eg, = torch.autograd.grad(e.sum(), both)
         assert torch.equal(y, e) and torch.equal(g, eg)
         del e, eg
+
+
+@pytest.mark.parametrize("M,D,dtype", [(20011, 128, "fp32"), (20011, 300, "fp32"), (5003, 2048, "fp32"), (20011, 333, "bf16"),
+                                       (9001, 1000, "bf16"), (5003, 2048, "bf16"), (30001, 100, "fp16")])
+def test_relu_backward_of_many_rows(M, D, dtype):
+    """The form a normed GCN_FC trains with, over more rows than the grid takes at once: one and two rows a lane group
+    at a time, with and without the next rows loaded ahead."""
+    case = _inputs(M, D, T[dtype], torch.float32, relu=True)
+    out = _run(*case, True)
+    _check(*case, True, out)
+    again = _run(*case, True)
+    assert all(torch.equal(a, b) for a, b in zip(out, again))
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("M,D,dtype", [(3001, 2500, "fp32"), (2051, 2049, "bf16"), (70001, 3, "fp32"), (70001, 5, "bf16"),
+                                       (70001, 1, "fp16")])
+def test_many_rows_of_a_block_each(M, D, dtype, relu):
+    """Rows longer than 2048 or shorter than a vector, more of them than blocks: the blocks' second rows, the weight
+    gradients' second row a grid row, the fold of all partial rows."""
+    case = _inputs(M, D, T[dtype], torch.float32, relu=relu)
+    out = _run(*case, relu)
+    _check(*case, relu, out)
+    again = _run(*case, relu)
+    assert all(torch.equal(a, b) for a, b in zip(out, again))
