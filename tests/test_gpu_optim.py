@@ -551,3 +551,26 @@ def test_a_refused_step_updates_nothing(bits):
             o.step()
         assert torch.equal(a, torch.ones_like(a)) and o.state[a]["step"] == 0 and o.last_norm is None
         assert not any(t.float().any() for t in o.state[a].values() if isinstance(t, torch.Tensor))
+
+
+def test_8bit_second_moment_at_the_default_beta():
+    """b2 = 0.999, where a step changes r by less than half a step of its format and rounding to nearest would keep it
+    for good: after 3000 steps of noise v is the 32-bit one's on average.  What random rounding adds: a stored r lies on
+    the format's grid, so a step of the grid (at most r / 8) and the distance d to a grid point give it the variance of
+    at most d r / 8, d at most r's change plus that of the block's scale, each (1 - b2) / 2 E|g^2 / v - 1| r, the
+    expectation 0.97 of a normal g: v gains 0.121 (1 - b2) v a step and forgets 1 - b2 of it, so its mean ratio is
+    between 1 and 1.121.  An element's ratio spreads by less than 0.5 (v itself by 0.03): 5 standard errors are 0.04."""
+    from lpgnn import optim
+
+    n = 4096
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    spread = 2.0 ** (-4 * torch.rand(n, generator=gen, device=DEV))  # (all of a block within the format's normal range)
+    p8, p32, m, v = (torch.zeros(n, device=DEV) for _ in range(4))
+    m8, r8 = (torch.zeros(n, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for _ in range(2))
+    ms, rs = (torch.zeros(n // 256, device=DEV) for _ in range(2))
+    for t in range(1, 3001):
+        g = torch.randn(n, generator=gen, device=DEV) * spread
+        optim.adamw_step_8bit([p8], [g], [m8], [ms], [r8], [rs], step=t, seed=2, **H)
+        optim.adamw_step([p32], [g], [m], [v], step=t, **H)
+    ratio = (r8.float() * rs.repeat_interleave(256)).square() / v
+    assert 0.96 < ratio.mean().item() < 1.17 and ratio.std().item() < 0.5
