@@ -236,3 +236,60 @@ def test_the_shallowest_model():
     lc, lv = model(batch)
     (rc, rv), _ = _model64(model, batch, A)  # (bound: test_forward_and_gradients)
     assert (lc.cpu().double() - rc).abs().max() < 1e-3 and (lv.cpu().double() - rv).abs().max() < 1e-3
+
+
+@pytest.mark.parametrize("seed,hids", [(5, 64), (6, 128)])
+def test_int8_evaluation_stays_near_full_precision(seed, hids):
+    """How far 8 bits move the model from its definition in 64 bits.  A code is off by at most half a unit, so a hidden
+    pre-activation by d = sum_k +- (s/2) |w_k| +- (ws/2) |x_k|: certainly below the sum of magnitudes, and, the roundings
+    being unrelated, below t = 6.5 root sum squares (Hoeffding: 1.3e-9 each; fp32's own 1e-5 is far below t / 6).  Heads
+    and logits follow: the roundings of a row through W_head, a hidden number that t can push across the ReLU's corner
+    counted in full; 10 h / |h| moves by at most 20 |dh| / |h|.  Where the two best logits are further apart than twice
+    that the answer is the same one."""
+    import i8_ref as R
+    from lpgnn import GCN_FC
+    from lpgnn.conv import two_direction_i8
+
+    batch, A = _batch(seed=seed)
+    torch.manual_seed(2)
+    model = GCN_FC(8, 8, hids=hids, depth=3).to(DEV).eval()
+    with torch.no_grad():
+        got = model.quantize_int8()(batch)
+        l1, r1 = model.conv1(batch.x_s, batch.x_t, batch.edge_index, relu=True)
+        hidden = two_direction_i8(l1, r1, batch.edge_index, model._int8[0], False)
+    sd = {k: v.double().cpu() for k, v in model.state_dict().items()}
+    left, right = batch.x_s.double().cpu(), batch.x_t.double().cpu()
+
+    def parts(pre, agg, own):
+        return torch.cat((agg, own), 1), torch.cat((sd[pre + ".lin_rel.weight"], sd[pre + ".lin_root.weight"]), 1), \
+            sd[pre + ".lin_rel.bias"]
+
+    def lin(x, W, b):
+        return x @ W.t() + b
+
+    l1, r1 = (lin(*parts("conv1.right2left", A @ right, left)).clamp(min=0),
+              lin(*parts("conv1.left2right", A.t() @ left, right)).clamp(min=0))
+    sides = (("layers.0.right2left", A @ r1, l1, "lin_left", left, hidden[0], got[0]),
+             ("layers.0.left2right", A.t() @ l1, r1, "lin_right", right, hidden[1], got[1]))
+    for pre, agg, own, head, feas, z8, logits in sides:
+        x, W, b = parts(pre, agg, own)
+        s, ws = (R.quantize(t.float())[1].double()[:, None] / 2 for t in (x, W))
+        xq = x.abs() + s  # (no less than what the codes stand for)
+        z = lin(x, W, b)
+        dz = (z8.double().cpu() - z).abs()
+        assert (dz <= s * W.abs().sum(1) + xq.sum(1, keepdim=True) * ws.t() + 1e-5).all()
+        t = 6.5 * (s.square() * W.square().sum(1) + xq.square().sum(1, keepdim=True) * ws.square().t()).sqrt()
+        assert (dz <= t).all() and t.median() < 0.2 * z.abs().median()
+        Wh = sd[head + ".weight"]
+        on, corner = (z > t).double(), (z.abs() <= t).double()
+        h = z.clamp(min=0) @ Wh.t() + sd[head + ".bias"]
+        dh = torch.stack([6.5 * (((on * w) @ W).square().sum(1) * s[:, 0].square()
+                                 + (on * w).square() @ ws[:, 0].square() * xq.square().sum(1)).sqrt()
+                          + (corner * t) @ w.abs() for w in Wh], 1)
+        bound = 20 * dh.norm(dim=1) / h.norm(dim=1)
+        y = 10 * h / h.norm(dim=1, keepdim=True)
+        y = y - 10 * torch.stack((feas[:, -3] != 0, torch.zeros(len(feas)).bool(), feas[:, -1] != 0), 1).double()
+        assert ((logits.double().cpu() - y).abs() <= bound[:, None] + 1e-3).all()
+        best = y.topk(2, 1).values
+        sure = best[:, 0] - best[:, 1] > 2 * bound
+        assert sure.any() and torch.equal(logits.cpu().argmax(1)[sure], y.argmax(1)[sure])
