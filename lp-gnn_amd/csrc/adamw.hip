@@ -23,8 +23,9 @@
 // 67 M numbers: 277 us with fp32 moments (6.8 TB/s), 166-186 with 8-bit ones (5.8), the norm 46 (5.8); 4.2 M: 8-bit
 // step 15, norm 5 + 4; 70 K in 22 tensors 4.2 us.
 //
-// The norm is summed in 64 bits: products of fp32 numbers are exact there, and the sum's order does not
-// show in the 32-bit result, so the clip factor is the same however the tensors are split.
+// The norm is summed in 64 bits, where products of fp32 numbers are exact, in a fixed order: the same list
+// gives the same bits.  Split otherwise, the sums differ in their last 64-bit places, so the norm and the
+// factor are the same 32-bit numbers or, where a border lies between them, neighbours.
 #include "common.h"
 #include "fc_common.h"  // lowbias32
 

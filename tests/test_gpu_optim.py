@@ -574,3 +574,17 @@ def test_8bit_second_moment_at_the_default_beta():
         optim.adamw_step([p32], [g], [m], [v], step=t, **H)
     ratio = (r8.float() * rs.repeat_interleave(256)).square() / v
     assert 0.96 < ratio.mean().item() < 1.17 and ratio.std().item() < 0.5
+
+
+def test_the_clip_under_other_splits_is_at_most_a_neighbour():
+    """The 64-bit sums of other splits differ by n 2^-53 of themselves at most, far below a step of fp32: the rounded
+    norm and factor are equal or neighbours, and the same list gives the same bits."""
+    from lpgnn import optim
+
+    g = torch.randn(3 * 2**20 + 77, generator=torch.Generator(device=DEV).manual_seed(9), device=DEV)
+    near = lambda a, b: abs(a.view(torch.int32).item() - b.view(torch.int32).item()) <= 1
+    whole = optim.clip_scale([g], 0.37)
+    assert all(torch.equal(a, b) for a, b in zip(whole, optim.clip_scale([g], 0.37)))
+    for k in (1, 5, 4096, 100003, 2**20):
+        for pieces in ([g[:k], g[k:]], list(g.split(max(k, 50021)))):
+            assert all(near(a, b) for a, b in zip(whole, optim.clip_scale(pieces, 0.37)))
