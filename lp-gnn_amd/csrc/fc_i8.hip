@@ -658,7 +658,7 @@ __global__ __launch_bounds__(256) void fc_i8_row(RowsArgs a) {
 // Some rows: a block of eight waves takes 16 rows and 128 columns.  It quantises its rows into LDS, two a wave
 // (every block of the row tile again), then each wave runs 16 columns with w's fragments straight from memory,
 // eight k steps in flight: no barrier and no second launch, which is what a call of this size consists of.
-constexpr int kSomeK = 1280;  // its longest row (16 of them and 16 bytes each in LDS)
+constexpr int kSomeK = 1024;  // its longest row (16 of them and 16 bytes each in LDS)
 constexpr int kSomeN = 128;
 template <typename T, int NV>
 __global__ __launch_bounds__(512) void fc_i8_some(RowsArgs a) {
@@ -797,19 +797,18 @@ lpg_status run_rows(const RowsArgs &a, hipStream_t s) {
                          16 * ((K + 511) / 512 * 512 + 16), s, a);
     };
     if (nv <= 1) go(fc_i8_some<T, 1>);
-    else if (nv <= 2) go(fc_i8_some<T, 2>);
-    else if (nv <= 4 || sizeof(T) == 2) go(fc_i8_some<T, 4>);  // (16 bits: at most 160 vectors)
-    else if constexpr (sizeof(T) == 4) go(fc_i8_some<T, 5>);   // (at most 320)
+    else if (nv <= 2 || sizeof(T) == 2) go(fc_i8_some<T, 2>);  // (16 bits: at most 128 vectors)
+    else if constexpr (sizeof(T) == 4) go(fc_i8_some<T, 4>);   // (at most 256)
   }
   LPG_HIP(hipGetLastError());
   return LPG_OK;
 }
 
-// What lpg_fc_i8_rows takes: one row that fits its LDS; some rows up to 1280 columns long, as many blocks as CUs at
-// most.  Then it is ahead of the two launches at every size (2 x 128, K = 128 5.1 us against 6.9; 512 x 1024, K = 1024
-// 8.0 and 9.4; 4000 x 100, K = 1024 7.8 and 12.0); of longer rows the two are faster (256 x 1024, K = 2048 13.0 and
-// 10.6), and with more blocks the rows that each quantises again cost more than the launch (2000 x 512, K = 256 13.6
-// and 7.3).
+// What lpg_fc_i8_rows takes: one row that fits its LDS; some rows up to 1024 columns long, as many blocks as CUs at
+// most.  Then it is ahead of the two launches at every M (fp16, N = 1024: K = 512 5.0 us against 7.6 for 2 rows, 5.6 and
+// 8.4 for 256; K = 1024 6.2 and 7.8 for 2, 7.2 and 8.8 for 64, 7.6 and 8.8 for 256).  Of longer rows the two are, at every
+// M too (K = 1040 9.1 and 7.6 for 2, 10.1 and 8.9 for 128; K = 2048 10.6 and 9.2, 11.7 and 10.4).  With more blocks
+// the rows that each quantises again cost more than the launch (2000 x 512, K = 256 13.6 and 7.3).
 bool few_rows(int64_t M, int64_t N, int64_t K) {
   if (M <= 1) return (K + 1023) / 1024 * 1024 <= kRowBytes && (N + 3) / 4 <= most_blocks(256);
   return K <= kSomeK && (M + 15) / 16 <= 65535 && (M + 15) / 16 * ((N + kSomeN - 1) / kSomeN) <= device_cus();

@@ -314,3 +314,12 @@ def test_more_rows_than_a_launch_holds():
         q0, s0 = quantize_i8(x[a:b].clone(), x2[a:b].clone())
         assert torch.equal(q[a:b], q0) and torch.equal(s[a:b], s0)
     assert s.count_nonzero() == 300
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("K1,K2", [(1024, 0), (1025, 0), (512, 512), (1000, 24), (1000, 25), (3, 1021), (769, 0), (768, 0), (257, 0),
+                                   (500, 13)])
+def test_few_rows_of_every_vector_count(K1, K2, dtype):
+    """Both sides of the longest row that few rows take in one launch, and of the rows that a lane's vectors reach."""
+    for M in (2, 17):
+        _check(*_case(M, 130, K1, K2, T[dtype], seed=6), relu=False)

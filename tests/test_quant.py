@@ -97,3 +97,12 @@ def test_c_entry_of_one_row_refuses_more_blocks_than_a_launch_holds():
 
     p, N = 1 << 20, 1 << 26
     assert _lib.lib().lpg_fc_i8_rows(2, 1, N, 16, p, 16, 0, None, 0, p, 16, p, None, 0, p, N, None) == 3
+
+
+def test_c_entry_of_few_rows_ends_at_1024_columns():
+    from lpgnn import _lib
+
+    p = 1 << 20
+    rw = lambda M, K1, K2: _lib.lib().lpg_fc_i8_rows(2, M, 64, K1, p, K1, K2, p, K2, p, 4096, p, None, 0, p, 64, None)
+    for M in (2, 16, 64):
+        assert rw(M, 1025, 0) == rw(M, 1000, 25) == rw(M, 1, 1024) == 3
