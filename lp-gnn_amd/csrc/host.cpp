@@ -14,6 +14,7 @@
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
@@ -100,7 +101,9 @@ int64_t ld(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 c10::DataPtr workspace(int64_t bytes) { return c10::GetAllocator(c10::DeviceType::CUDA)->allocate((size_t)bytes); }
 
 // The operators have no forward-mode derivative: a dual tensor's tangent would be dropped, which reads as a derivative
-// of zero.
+// of zero.  (No tensor has one while no level of the mode is open: one look a call, not one a tensor -- 22 parameters'
+// lists 7.6 us with the latter, 6.2 with the former.)
+bool forward_mode() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 void no_tangent(const char *what, const Tensor &t) {
   REQUIRE(!t.defined() || !t._fw_grad(0).defined(), "lpgnn ", what, ": there is no forward-mode derivative");
 }
@@ -219,7 +222,8 @@ void no_eager_leaf(const Tensor &t) {
 
 Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double eps, bool relu) {
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
-  for (const Tensor *t : {&x, &w, &b}) no_tangent("layer_norm", *t);
+  if (forward_mode())
+    for (const Tensor *t : {&x, &w, &b}) no_tangent("layer_norm", *t);
   REQUIRE(x.is_cuda(), "lpgnn layer_norm: runs on a HIP device only (no CPU path)");
   REQUIRE(code_of(x.scalar_type()) >= 0, "lpgnn layer_norm: x must be float32, bfloat16 or float16, got ",
           x.scalar_type());
@@ -261,15 +265,20 @@ struct Tensors {
     if (!fast) throw pybind11::error_already_set();
     n = (size_t)PySequence_Fast_GET_SIZE(fast.ptr());
     items = PySequence_Fast_ITEMS(fast.ptr());
-    for (size_t i = 0; i < n; ++i) {
+    for (size_t i = 0; i < n; ++i)
       if (!THPVariable_Check(items[i])) throw pybind11::type_error(c10::str("lpgnn ", what, ": the lists hold tensors"));
-      no_tangent(what, (*this)[i]);
-    }
   }
   size_t size() const { return n; }
   bool empty() const { return n == 0; }
   const Tensor &operator[](size_t i) const { return THPVariable_Unpack(items[i]); }
 };
+
+void no_tangents(const char *what, std::initializer_list<const Tensors *> lists, const OptTensor &scale = std::nullopt) {
+  if (!forward_mode()) return;
+  for (const Tensors *ts : lists)
+    for (size_t i = 0; i < ts->size(); ++i) no_tangent(what, (*ts)[i]);
+  no_tangent(what, scale);
+}
 
 // `ts` beside the parameters `ps`: as many, one type, the parameters' device, contiguous, their sizes (or,
 // scales, one number a block of 256)
@@ -363,7 +372,7 @@ void adamw_step(handle params_, handle grads, handle exp_avgs, handle exp_avg_sq
   const char *what = "adamw_step";
   const Tensors ps(params_, what), gs(grads, what), ms(exp_avgs, what), vs(exp_avg_sqs, what);
   const lpg_adamw_hyper h = hyper(what, step, lr, betas, eps, weight_decay);
-  no_tangent(what, grad_scale);
+  no_tangents(what, {&ps, &gs, &ms, &vs}, grad_scale);
   if (ps.empty()) return;
   const int32_t type = params(what, ps);
   same(what, "grads", gs, ps, ps[0].scalar_type());
@@ -403,7 +412,7 @@ void adamw_step_8bit(handle params_, handle grads, handle m8_, handle m_scales, 
   const char *what = "adamw_step_8bit";
   const Tensors ps(params_, what), gs(grads, what), m8(m8_, what), ms(m_scales, what), r8(r8_, what), rs(r_scales, what);
   const lpg_adamw_hyper h = hyper(what, step, lr, betas, eps, weight_decay);
-  no_tangent(what, grad_scale);
+  no_tangents(what, {&ps, &gs, &m8, &ms, &r8, &rs}, grad_scale);
   if (ps.empty()) return;
   const int32_t type = params(what, ps);
   REQUIRE(!places || places->size() == ps.size(), "lpgnn ", what, ": ", ps.size(), " params and ", places->size(),
@@ -429,6 +438,7 @@ void adamw_step_8bit(handle params_, handle grads, handle m8_, handle m_scales, 
 std::pair<Tensor, Tensor> clip_scale(handle grads, double max_norm) {
   const char *what = "clip_scale";
   const Tensors gs(grads, what);
+  no_tangents(what, {&gs});
   REQUIRE(!gs.empty(), "lpgnn clip_scale: no gradients");
   REQUIRE(max_norm >= 0, "lpgnn clip_scale: max_norm must not be negative, got ", max_norm);
   const int32_t type = params(what, gs);
@@ -447,7 +457,7 @@ std::pair<Tensor, Tensor> clip_scale(handle grads, double max_norm) {
 // ------------------------------------------------------------------ 8-bit integers
 // whole numbers have no derivative: nothing a call computes from may want one
 void no_gradient(const char *what, const OptTensor &t) {
-  no_tangent(what, t);
+  if (forward_mode()) no_tangent(what, t);
   REQUIRE(!at::GradMode::is_enabled() || !t || !t->requires_grad(), "lpgnn ", what,
           ": 8-bit integers have no gradient (call it under torch.no_grad())");
 }
