@@ -15,9 +15,10 @@
 // fc_i8: MFMA- and LDS-bound (v_mfma_i32_16x16x64_i8), the k loop of the 16-bit kernel (fc_bf16.hip fc_bf16_p) on
 // bytes: 128-byte k tiles staged by buffer_load ... lds into a swizzled image, two buffers (four in the small tile),
 // one barrier a tile in its middle, fragment reads one half tile ahead, transposed fragments (W x A^T: a lane holds
-// four consecutive columns of one row), stores straight from registers.  16384 x 2048, K = 4096: 108 us, 2.55 POPS;
-// 100 K x 1024, K = 2048: 194 us, 2.16, and 170 behind the codes (in cache then).  A k tile takes 1.4 us, of which the
-// MFMAs 0.85 at 2.4 GHz; the first round's loads and the last one's stores are not hidden.
+// four consecutive columns of one row), stores straight from registers.  16384 x 2048, K = 4096: 109 us, 2.5 POPS;
+// 100 K x 1024, K = 2048: 184 us, 2.3 (170 of it the 256 tile, 13 the 128 tile of the last rows), with its codes 276.  160
+// k tiles of five output tiles in a row take a block 255 us, 1.6 us each with the stores, of which the MFMAs 0.86 at 2.4
+// GHz; the first round's loads and the last one's stores are not hidden.
 // fc_i8_row, fc_i8_some: few rows are bound by latency -- the second launch, the k loop's barriers -- and by
 // w's bytes: every block quantises its rows into LDS itself, its first loads of w in flight meanwhile.  One row of
 // 2048 to 1024 columns: 3.8 us.
@@ -851,8 +852,8 @@ extern "C" lpg_status lpg_quant_i8(int32_t dtype, int64_t M, int64_t K1, const v
   LPG_REQUIRE(ldq >= K1 + K2 && ldq % 128 == 0, "lpg_quant_i8: ldq must be a multiple of 128 that holds K1 + K2");
   LPG_REQUIRE(M == 0 || (x && q && scale && (K2 == 0 || x2)), "lpg_quant_i8: NULL pointer");
   LPG_REQUIRE(aligned16(q), "lpg_quant_i8: q must be 16-byte aligned");
-  // x past the caches where it would push out the codes (100 K x 2048 fp32 with the product to 1024 469 -> 394 us, 60 K x
-  // 2048 fp16 187 -> 177); a small x may still be in them (20000 x 1024 fp16 45 us through them, 47 past them)
+  // x past the caches where it would push out the codes (100 K x 2048 fp32 with the product to 1024 469 -> 394 us, 376 by now,
+  // 60 K x 2048 fp16 187 -> 177); a small x may still be in them (20000 x 1024 fp16 45 us through them, 47 past them)
   const int past = M * (K1 + K2) * (dtype == LPG_F32 ? 4 : 2) > (int64_t)128 << 20;
   const QuantArgs a{M, ldx, ldx2, ldq, (int)K1, (int)K2, x, x2, q, scale, past};
   const auto go = [&](auto kernel, int rows) -> lpg_status {

@@ -23,9 +23,10 @@
 // persistent grid), the block adds its waves' sums in wave order in LDS and writes one partial row, and
 // a second kernel adds the partial rows in block order: the same bits every run.
 //
-// Kernel times: forward 100 K x 1024 fp32 142 us (5.8 TB/s), 200 K x 2048 bf16 294 (5.6), 50001 x 1000 fp16 38
-// (5.3, rows off cache lines), 200 x 128 2.6; backward of the first two 218 (5.6 TB/s) and 416 (5.9), their folds
-// 5 and 4.
+// Kernel times: forward 100 K x 1024 fp32 143 us (5.7 TB/s), 200 K x 2048 bf16 297 (5.5), 50001 x 1000 fp16 41
+// (4.9, rows off cache lines), 200 x 128 2.8; backward of the first two 221 (5.6 TB/s) and 421 (5.8), with the ReLU 226
+// and 432, their folds 5.  A block a row is far from that: 50 K x 4096 bf16 526 us forward (1.6 TB/s), 1.3 ms with
+// the backward (1.3), 1.5 with the ReLU.
 #include "common.h"
 
 #include <type_traits>
