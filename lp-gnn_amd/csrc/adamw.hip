@@ -384,19 +384,18 @@ bool hyper_ok(const lpg_adamw_hyper &h) {
 // Fills tables of at most `many` tensors (those without elements left out) and launches each.
 template <typename Tab, typename E, typename L>
 lpg_status in_tables(Tab &tab, int many, int64_t chunk, int64_t count, const E *list, const char *what, L launch) {
+  for (int64_t i = 0; i < count; ++i)  // (before the first launch: a refused call updates nothing)
+    if (blocks_of(list[i].n, chunk) > most_blocks(kT)) {
+      set_error("%s: a tensor of %lld elements is too large", what, (long long)list[i].n);
+      return LPG_ERR_UNSUPPORTED;
+    }
   for (int64_t at = 0; at < count;) {
     int k = 0;
     int64_t blocks = 0;
     for (; at < count && k < many; ++at) {
       if (list[at].n == 0) continue;
       const int64_t b = blocks_of(list[at].n, chunk);
-      if (blocks + b > most_blocks(kT)) {
-        if (k == 0) {
-          set_error("%s: a tensor of %lld elements is too large", what, (long long)list[at].n);
-          return LPG_ERR_UNSUPPORTED;
-        }
-        break;
-      }
+      if (blocks + b > most_blocks(kT)) break;
       tab.t[k] = list[at];
       tab.first[k++] = (uint32_t)blocks;
       blocks += b;

@@ -220,3 +220,18 @@ def test_c_entries_refuse_more_blocks_than_a_launch_holds():
     assert L.lpg_adamw8(2, 1, i64(p, p, p, p, p, p, 1 << 34, 0), h, None, None) == 3
     assert b"too large" in L.lpg_last_error()
     assert L.lpg_grad_norm(2, 1, i64(p, 1 << 38), 1.0, p, p, p, None) == 3 and b"too large" in L.lpg_last_error()
+
+
+def test_c_entries_refuse_before_the_first_launch():
+    """A tensor too large behind others that are not: nothing of the call may run (here a launch would be error 2)."""
+    import ctypes
+
+    from lpgnn import _lib
+
+    L = _lib.lib()
+    h = _lib.LpgAdamwHyper(0.9, 0.1, 0.999, 0.001, 1.0, 1e-8, 1.0, 1e-3)
+    p = 1 << 20  # never dereferenced
+    i64 = lambda *a: (ctypes.c_int64 * len(a))(*a)
+    assert L.lpg_adamw(2, 2, i64(p, p, p, p, 4, p, p, p, p, 1 << 36), h, None, None) == 3
+    assert L.lpg_adamw8(2, 2, i64(p, p, p, p, p, p, 4, 0, p, p, p, p, p, p, 1 << 34, 0), h, None, None) == 3
+    assert L.lpg_grad_norm(2, 2, i64(p, 4, p, 1 << 38), 1.0, p, p, p, None) == 3
