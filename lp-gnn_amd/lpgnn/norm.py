@@ -23,7 +23,8 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
                relu: bool = False) -> Tensor:
     """act((x - mean) / sqrt(var + eps) * weight + bias) over the last dimension of x (weight None = ones,
     bias None = zeros, act = ReLU with ``relu``).  A row that holds a NaN or an infinity comes out as NaN;
-    other rows are not touched by it."""
+    other rows are not touched by it.  The squares are summed in fp32: of a row whose sum of squared deviations passes
+    its range (3.4e38) only the bias is left."""
     tok = TIMER.start(("layer_norm", tuple(x.shape), str(x.dtype)[6:])) if TIMER.enabled else None
     y = _lib.host().layer_norm(x, weight, bias, eps, relu)
     TIMER.stop(tok)

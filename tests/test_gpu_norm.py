@@ -387,3 +387,15 @@ def test_many_rows_of_a_block_each(M, D, dtype, relu):
     _check(*case, relu, out)
     again = _run(*case, relu)
     assert all(torch.equal(a, b) for a, b in zip(out, again))
+
+
+def test_rows_past_the_range_of_their_squares():
+    """Finite rows whose sum of squares no fp32 number holds come out as the bias; the ones beside them do not notice."""
+    from lpgnn import layer_norm
+
+    for D in (64, 300, 2100):
+        x, w, b, _ = (t.to(DEV) for t in _inputs(5, D, torch.float32, torch.float32))
+        clean = layer_norm(x, w, b, EPS)
+        x[3] = x[3] / x[3].abs().max() * 1e22
+        y = layer_norm(x, w, b, EPS)
+        assert torch.equal(y[3], b) and torch.equal(y[[0, 1, 2, 4]], clean[[0, 1, 2, 4]])
