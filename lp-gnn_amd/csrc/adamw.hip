@@ -385,7 +385,7 @@ bool hyper_ok(const lpg_adamw_hyper &h) {
 template <typename Tab, typename E, typename L>
 lpg_status in_tables(Tab &tab, int many, int64_t chunk, int64_t count, const E *list, const char *what, L launch) {
   for (int64_t i = 0; i < count; ++i)  // (before the first launch: a refused call updates nothing)
-    if (blocks_of(list[i].n, chunk) > most_blocks(kT)) {
+    if (list[i].n > most_blocks(kT) * chunk) {
       set_error("%s: a tensor of %lld elements is too large", what, (long long)list[i].n);
       return LPG_ERR_UNSUPPORTED;
     }
